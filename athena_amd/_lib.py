@@ -189,6 +189,15 @@ _SIGNATURES = {
     "athena_cast": (c_int, [_P, c_int, _P, c_int, c_long, _S]),
     "athena_copy_many": (c_int, [_P, _P, _P, c_int, _S]),
     "athena_axpby": (c_int, [c_float, _P, c_float, _P, c_long, c_int, _S]),
+    "athena_kv_plan": (c_int, [_P, _P, _P, c_long, c_int, _P, c_int, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _S]),
+    "athena_kv8_append": (c_int, [_P, _P, c_long, c_long, c_long, c_long, c_int, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int,
+                                  c_int, c_int, _S]),
+    "athena_kv8_attention_workspace_bytes": (c_int64, [c_int] * 9),
+    "athena_kv8_attention": (c_int, [_P, c_long, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_int, _P, c_long, c_int, _P, _P,
+                                     c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_long, c_long, _P, _P,
+                                     c_int64, _S]),
+    "athena_logits_process": (c_int, [_P, c_long, c_int, c_int, c_int, _P, c_long, c_int, _P, _P, _P, _P, _P, c_long, _P,
+                                      c_long, _P, c_long, c_int, _P, c_long, _P, c_long, _S]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,445 @@
+// Paged key/value cache in 8 bits for decoding: block plans (which blocks a request gets, where its new
+// tokens go), the write of new keys and values, and attention over the cache.
+//
+// The cache of one attention layer, in blocks of ``block_size`` tokens:
+//   k_codes int8 [blocks][kv_heads][block_size][width]   k_scale fp32 [blocks][kv_heads]
+//   v_codes int8 [blocks][kv_heads][width][block_size]   v_scale fp32 [blocks][kv_heads]
+// An element stands for code * scale.  Keys are contracted over the head's columns and lie row by row, values
+// are contracted over the tokens and lie column by column: both are then read from memory straight into
+// matrix-core operands, without a transposition on the way.
+#include "common.h"
+
+// ---------------------------------------------------------------- block plans
+// One workgroup sums over the requests (new rows, blocks taken, blocks given back), decides whether the
+// plan fits, and leaves the running sums; rows, table entries and returned blocks are then filled in by
+// ``plan_fill``, in the same workgroup or in a launch of many.  Whole numbers throughout.
+#define PLAN_THREADS 1024
+
+struct PlanArgs {
+    const int32_t* lens;
+    const int32_t* new_rows;
+    int32_t* tables;
+    long ld_tables;
+    int32_t* free_blocks;
+    const int32_t* free_count;
+    int32_t *cu_rows, *slots, *positions, *lens_out, *free_count_out, *status;
+    int32_t* work;          // [2][B] first block taken / given back by a request, then {blocks in the stack, level, fits}
+    int32_t* before;        // [B] lengths before the plan
+    int B, table_width, free_capacity, block_size, rows;
+};
+
+struct PlanSum {
+    long long rows;
+    long long taken, given;
+};
+
+__device__ __forceinline__ long long shfl_up64(long long v, int o) { return __shfl_up(v, o, 64); }
+
+// blocks of n tokens
+__device__ __forceinline__ int blocks_of(long long n, int bs) { return (int)((n + bs - 1) / bs); }
+
+__device__ __forceinline__ int plan_stack(const PlanArgs& a, int count, int at) {
+    // entry ``at`` of the stack of free blocks with the given-back ones on top of it
+    if (at < count) return a.free_blocks[at];
+    const int32_t* given = a.work + a.B;
+    const int f = at - count;
+    int lo = 0, hi = a.B - 1;                   // last request whose first given-back block is <= f
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (given[mid] <= f) lo = mid;
+        else hi = mid - 1;
+    }
+    return a.tables[(long)lo * a.ld_tables + (f - given[lo])];
+}
+
+// threads [first, first + step, ...) of the rows, waves [first / 64, ...) of the requests
+__device__ __forceinline__ void plan_fill(const PlanArgs& a, int first, int step) {
+    const int32_t* end = a.work + 2 * a.B;
+    const int count = end[0], level = end[1], fits = end[2];
+    const int total = fits ? a.cu_rows[a.B] : 0;
+    for (int t = first; t < a.rows; t += step) {
+        int slot = -1, pos = 0;
+        if (t < total) {
+            int lo = 0, hi = a.B - 1;           // last request that begins at or before row t
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (a.cu_rows[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int len = a.before[lo];
+            pos = len + t - a.cu_rows[lo];
+            const int j = pos / a.block_size, have = blocks_of(len, a.block_size);
+            const int block = j < have ? a.tables[(long)lo * a.ld_tables + j]
+                                       : plan_stack(a, count, level - 1 - (a.work[lo] + j - have));
+            slot = block < 0 ? -1 : block * a.block_size + pos % a.block_size;
+        }
+        a.slots[t] = slot;
+        a.positions[t] = pos;
+    }
+    if (!fits) return;
+    const int lane = first & 63;
+    for (int b = first >> 6; b < a.B; b += step >> 6) {
+        const int len = a.before[b], n = a.new_rows[b];
+        const int have = blocks_of(len, a.block_size);
+        int32_t* row = a.tables + (long)b * a.ld_tables;
+        if (n < 0) {
+            const int at = count + a.work[a.B + b];
+            for (int j = lane; j < have; j += 64) a.free_blocks[at + j] = row[j];
+        } else {
+            const int need = blocks_of((long long)len + n, a.block_size) - have;
+            for (int j = lane; j < need; j += 64) row[have + j] = plan_stack(a, count, level - 1 - (a.work[b] + j));
+        }
+    }
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void kv_plan_kernel(PlanArgs a, int fill) {
+    __shared__ PlanSum part[PLAN_THREADS / 64];
+    __shared__ int s_long, s_fits;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int per = (a.B + PLAN_THREADS - 1) / PLAN_THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    if (tid == 0) s_long = 0;
+    __syncthreads();
+    PlanSum mine = {0, 0, 0};
+    int too_long = 0;
+    const long long top = (long long)a.table_width * a.block_size;
+    for (int b = b0; b < b1; ++b) {
+        const int len = a.lens[b], n = a.new_rows[b];
+        if (len < 0 || (long long)len + max(n, 0) > top) {
+            ++too_long;
+            continue;
+        }
+        const int have = blocks_of(len, a.block_size);
+        if (n < 0) mine.given += have;
+        else {
+            mine.rows += n;
+            mine.taken += blocks_of((long long)len + n, a.block_size) - have;
+        }
+    }
+    if (too_long) atomicAdd(&s_long, too_long);
+    PlanSum run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long r = shfl_up64(run.rows, o), t = shfl_up64(run.taken, o), g = shfl_up64(run.given, o);
+        if (lane >= o) { run.rows += r; run.taken += t; run.given += g; }
+    }
+    if (lane == 63) part[w] = run;
+    __syncthreads();
+    PlanSum base = {0, 0, 0}, all = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < PLAN_THREADS / 64; ++i) {
+        if (i < w) { base.rows += part[i].rows; base.taken += part[i].taken; base.given += part[i].given; }
+        all.rows += part[i].rows; all.taken += part[i].taken; all.given += part[i].given;
+    }
+    int32_t* end = a.work + 2 * a.B;
+    if (tid == 0) {
+        const int count = min(max(a.free_count[0], 0), a.free_capacity);
+        const long long level = count + all.given;
+        const long long missing = max(all.taken - level, 0ll), rows_over = max(all.rows - a.rows, 0ll),
+                        stack_over = max(level - a.free_capacity, 0ll);
+        const int fits = !(s_long || missing || rows_over || stack_over);
+        const long long most = 0x7fffffff;
+        a.status[0] = (int)min(missing, most);
+        a.status[1] = s_long;
+        a.status[2] = (int)min(rows_over, most);
+        a.status[3] = (int)min(stack_over, most);
+        end[0] = count;
+        end[1] = fits ? (int)level : count;
+        end[2] = fits;
+        s_fits = fits;
+        a.cu_rows[a.B] = fits ? (int)all.rows : 0;
+        a.free_count_out[0] = fits ? (int)(level - all.taken) : a.free_count[0];
+    }
+    __syncthreads();
+    const int fits = s_fits;
+    long long rows = base.rows + run.rows - mine.rows, taken = base.taken + run.taken - mine.taken,
+              given = base.given + run.given - mine.given;
+    for (int b = b0; b < b1; ++b) {
+        const int len = a.lens[b], n = a.new_rows[b];
+        a.before[b] = len;
+        a.cu_rows[b] = fits ? (int)rows : 0;
+        a.work[b] = (int)taken;
+        a.work[a.B + b] = (int)given;
+        a.lens_out[b] = !fits ? len : n < 0 ? 0 : len + n;
+        if (!fits) continue;
+        const int have = blocks_of(len, a.block_size);
+        if (n < 0) given += have;
+        else {
+            rows += n;
+            taken += blocks_of((long long)len + n, a.block_size) - have;
+        }
+    }
+    if (!fill) return;
+    __threadfence_block();
+    __syncthreads();
+    plan_fill(a, tid, PLAN_THREADS);
+}
+
+__global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a) {
+    plan_fill(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+extern "C" int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int32_t* tables, long ld_tables, int table_width,
+                              int32_t* free_blocks, int free_capacity, const int32_t* free_count, int B, int block_size,
+                              int rows, int32_t* cu_rows, int32_t* slots, int32_t* positions, int32_t* lens_out,
+                              int32_t* free_count_out, int32_t* status, int32_t* work, athena_stream_t stream) {
+    ATHENA_REQUIRE(B > 0 && table_width > 0 && free_capacity > 0 && rows >= 0 && ld_tables >= table_width, ATHENA_E_SHAPE,
+                   "athena_kv_plan: bad shape B=%d table_width=%d free_capacity=%d rows=%d ld=%ld", B, table_width,
+                   free_capacity, rows, ld_tables);
+    ATHENA_REQUIRE(block_size == 16 || block_size == 32 || block_size == 64 || block_size == 128, ATHENA_E_UNSUPPORTED,
+                   "athena_kv_plan: block size %d not in {16, 32, 64, 128}", block_size);
+    ATHENA_REQUIRE((long)table_width * block_size < (1L << 31), ATHENA_E_SHAPE, "athena_kv_plan: table too wide");
+    ATHENA_REQUIRE(lens && new_rows && tables && free_blocks && free_count && cu_rows && (slots || !rows) && (positions || !rows) &&
+                       lens_out && free_count_out && status && work,
+                   ATHENA_E_SHAPE, "athena_kv_plan: null operand");
+    PlanArgs a = {lens, new_rows, tables, ld_tables, free_blocks, free_count, cu_rows, slots, positions, lens_out,
+                  free_count_out, status, work, work + 2L * B + 3, B, table_width, free_capacity, block_size, rows};
+    hipStream_t s = (hipStream_t)stream;
+    const int fill = 1;
+    ATHENA_LAUNCH(kv_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, s, a, fill);
+    ATHENA_CHECK_LAUNCH("athena_kv_plan");
+    return ATHENA_OK;
+}
+
+// ---------------------------------------------------------------- writing new keys and values
+// A run of consecutive rows that go to the same block is one unit of work: the block's scale grows to the
+// largest magnitude of the run / 127 (from nothing where the run begins the block), codes already in the
+// block in front of the run are brought to a grown scale, and the run's codes are written.  One wave per
+// (run, kv head, keys or values); waves of one block never meet, as a run is taken by the wave that finds
+// its first row.
+//
+// Codes are round-half-to-even(x / scale) exactly: the product with the reciprocal in fp32 is off by less
+// than 127 * 2^-23, so a quotient within 1e-4 of a border is divided again in 64 bits, where quotients of
+// fp32 operands of this size cannot come closer than 2^-34 to a border without lying on it.
+template <typename T> struct AppendSide {
+    const T* x;
+    long ld_row, ld_head;
+    int8_t* codes;
+    float* scale;
+};
+
+__device__ __forceinline__ int code_of(float x, float s, float inv) {
+    const float f = x * inv;
+    float q = rintf(f);
+    if (fabsf(fabsf(f - q) - 0.5f) < 1e-4f || s < 1e-30f) q = s > 0.f ? (float)rint((double)x / (double)s) : 0.f;
+    return (int)fminf(fmaxf(q, -127.f), 127.f);             // (NaN: -127 or 127; the scale is NaN then)
+}
+__device__ __forceinline__ int recode(int q, float s0, float s1, float ratio) {
+    const float f = (float)q * ratio;
+    float r = rintf(f);
+    if (fabsf(fabsf(f - r) - 0.5f) < 1e-4f || s0 < 1e-30f) r = (float)rint((double)q * (double)s0 / (double)s1);
+    return (int)r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendSide<T> ks, AppendSide<T> vs, const int32_t* __restrict__ slots,
+                                                         int N, int rows_per_wg, int hk, int dk, int width, int block_size,
+                                                         long slots_end) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, head = blockIdx.y;
+    const int t0 = blockIdx.x * rows_per_wg;
+    // first rows of runs among the workgroup's rows
+    bool leads = false;
+    if (lane < rows_per_wg && t0 + lane < N) {
+        const int s = slots[t0 + lane], p = t0 + lane > 0 ? slots[t0 + lane - 1] : -1;
+        leads = s >= 0 && s < slots_end && !(p >= 0 && p < slots_end && p / block_size == s / block_size);
+    }
+    unsigned long long found = __ballot(leads);
+    int job = 0;
+    while (found) {
+        const int t = t0 + __ffsll((long long)found) - 1;
+        found &= found - 1;
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side, ++job) {
+            if (job % nw != w) continue;
+            const AppendSide<T> a = side ? vs : ks;
+            const int block = slots[t] / block_size;
+            // the run's length and first place
+            int n = 0, place = block_size;
+            for (;; n += 64) {
+                const int s = t + n + lane < N ? slots[t + n + lane] : -1;
+                const bool in = s >= 0 && s < slots_end && s / block_size == block;
+                const unsigned long long same = __ballot(in);
+                const int len = same == ~0ull ? 64 : __ffsll((long long)~same) - 1;
+                int p = lane < len ? s % block_size : block_size;
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) p = min(p, __shfl_xor(p, o, 64));
+                place = min(place, p);
+                if (len < 64) { n += len; break; }
+            }
+            const T* x = a.x + (long)t * a.ld_row + (long)head * a.ld_head;
+            unsigned top = 0;                   // largest magnitude, as bits: NaN over infinity over numbers
+            for (int e = lane; e < n * dk; e += 64) {
+                const int r = e / dk, c = e - r * dk;
+                top = max(top, __float_as_uint(to_f32<T>(x[(long)r * a.ld_row + c])) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
+            const long at = (long)block * hk + head;
+            const float s0 = place == 0 ? 0.f : a.scale[at], s1n = __uint_as_float(top) / 127.f;
+            // (as whole numbers, so that a scale that is NaN stays)
+            const float s1 = __uint_as_float(max(__float_as_uint(s0) & 0x7fffffffu, __float_as_uint(s1n) & 0x7fffffffu));
+            int8_t* codes = a.codes + at * (long)width * block_size;
+            const int row = side ? 1 : width, col = side ? block_size : 1;      // steps of a token / a column
+            if (s1 > s0 && place > 0) {
+                const float ratio = s0 / s1;
+                for (int e = lane; e < place * width; e += 64) {
+                    const int r = e / width, c = e - r * width;
+                    int8_t* p = codes + (long)r * row + (long)c * col;
+                    *p = (int8_t)recode(*p, s0, s1, ratio);
+                }
+            }
+            const float inv = s1 > 0.f ? 1.f / s1 : 0.f;
+            for (int e = lane; e < n * width; e += 64) {
+                const int r = e / width, c = e - r * width;
+                const int off = slots[t + r] % block_size;
+                const float v = c < dk ? to_f32<T>(x[(long)r * a.ld_row + c]) : 0.f;
+                codes[(long)off * row + (long)c * col] = (int8_t)code_of(v, s1, inv);
+            }
+            if (lane == 0) a.scale[at] = s1;
+        }
+    }
+}
+
+static int kv8_check(const char* name, int num_blocks, int hk, int block_size, int dk, int width) {
+    ATHENA_REQUIRE(num_blocks > 0 && hk > 0 && hk <= 65535 && dk > 0 && dk <= width, ATHENA_E_SHAPE,
+                   "%s: bad shape blocks=%d kv_heads=%d head=%d width=%d", name, num_blocks, hk, dk, width);
+    ATHENA_REQUIRE(block_size == 16 || block_size == 32 || block_size == 64 || block_size == 128, ATHENA_E_UNSUPPORTED,
+                   "%s: block size %d not in {16, 32, 64, 128}", name, block_size);
+    ATHENA_REQUIRE(width == 32 || width == 64 || width == 128, ATHENA_E_UNSUPPORTED, "%s: width %d not in {32, 64, 128}", name,
+                   width);
+    ATHENA_REQUIRE((long)num_blocks * block_size < (1L << 31), ATHENA_E_SHAPE, "%s: more than 2^31 places", name);
+    return ATHENA_OK;
+}
+
+extern "C" int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, long ldv, long ldv_head, int dtype,
+                                 const int32_t* slots, int N, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
+                                 int num_blocks, int hk, int block_size, int dk, int width, athena_stream_t stream) {
+    int rc = kv8_check("athena_kv8_append", num_blocks, hk, block_size, dk, width);
+    if (rc) return rc;
+    ATHENA_REQUIRE(N >= 0, ATHENA_E_SHAPE, "athena_kv8_append: N=%d", N);
+    if (N == 0) return ATHENA_OK;
+    ATHENA_REQUIRE(k && v && slots && k_codes && v_codes && k_scale && v_scale, ATHENA_E_SHAPE, "athena_kv8_append: null operand");
+    ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN, "athena_kv8_append: codes must lie on 16 bytes");
+    ATHENA_REQUIRE(dtype == ATHENA_F32 || dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_append: dtype");
+    const int per = (long)N * hk <= 4096 ? 1 : 16;
+    const dim3 grid((N + per - 1) / per, hk), block(per == 1 ? 128 : 256);
+    const long end = (long)num_blocks * block_size;
+    if (dtype == ATHENA_BF16) {
+        AppendSide<bf16_t> ks = {(const bf16_t*)k, ldk, ldk_head, k_codes, k_scale}, vs = {(const bf16_t*)v, ldv, ldv_head, v_codes, v_scale};
+        ATHENA_LAUNCH(kv8_append_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, width, block_size, end);
+    } else {
+        AppendSide<float> ks = {(const float*)k, ldk, ldk_head, k_codes, k_scale}, vs = {(const float*)v, ldv, ldv_head, v_codes, v_scale};
+        ATHENA_LAUNCH(kv8_append_kernel<float>, grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, width, block_size, end);
+    }
+    ATHENA_CHECK_LAUNCH("athena_kv8_append");
+    return ATHENA_OK;
+}
+
+// ---------------------------------------------------------------- attention over the cache
+// out[t, head] = sum_j p_j v_j, p = softmax_j(scale * q_t . k_j) over the tokens j of t's sequence that it may
+// see.  One workgroup per (row, head); keys in tiles of 128: a thread scores one key, then the threads take
+// the columns of the output.
+struct KvAttn {
+    const void* q;
+    long ldq, ldq_head;
+    const int8_t *k_codes, *v_codes;
+    const float *k_scale, *v_scale;
+    const int32_t* tables;
+    long ld_tables;
+    const int32_t *lens, *cu_rows;
+    void* out;
+    long ldo, ldo_head;
+    float* lse;             // [N][heads] or null
+    int table_width, num_blocks, B, N, h, hk, dk, block_size, causal;
+    float scale;
+};
+
+#define KV_TILE 128
+
+template <typename T, int W>
+__global__ __launch_bounds__(KV_TILE) void kv8_attention_kernel(KvAttn a) {
+    __shared__ float sq[W], sp[KV_TILE], red[32];
+    const int b = blockIdx.z, head = blockIdx.y, tid = threadIdx.x;
+    const int lo = min(max(a.cu_rows ? a.cu_rows[b] : b, 0), a.N), hi = min(max(a.cu_rows ? a.cu_rows[b + 1] : b + 1, lo), a.N);
+    const long long most = (long long)a.table_width * a.block_size;
+    const int len = (int)min((long long)max(a.lens[b], 0), most), g = head / (a.h / a.hk);
+    for (int t = lo + blockIdx.x; t < hi; t += gridDim.x) {
+        const T* q = (const T*)a.q + (long)t * a.ldq + (long)head * a.ldq_head;
+        __syncthreads();
+        for (int c = tid; c < W; c += KV_TILE) sq[c] = c < a.dk ? to_f32<T>(q[c]) * a.scale : 0.f;
+        __syncthreads();
+        const int end = a.causal ? min(len, len - (hi - t) + 1) : len;
+        float m = -INFINITY, l = 0.f, o = 0.f;
+        for (int j0 = 0; j0 < end; j0 += KV_TILE) {
+            const int j = j0 + tid;
+            float s = -INFINITY;
+            if (j < end) {
+                const int block = a.tables[(long)b * a.ld_tables + j / a.block_size];
+                if (block >= 0 && block < a.num_blocks) {
+                    const long at = (long)block * a.hk + g;
+                    const int8_t* k = a.k_codes + (at * a.block_size + j % a.block_size) * W;
+                    s = 0.f;
+                    for (int c = 0; c < W; ++c) s = fmaf(sq[c], (float)k[c], s);
+                    s *= a.k_scale[at];
+                }
+            }
+            const float mn = fmaxf(m, block_max(s, red)), base = mn == -INFINITY ? 0.f : mn;
+            const float p = __expf(s - base), alpha = __expf(m - base);
+            sp[tid] = p;
+            l = l * alpha + block_sum(p, red);
+            __syncthreads();
+            o *= alpha;
+            if (tid < W) {
+                for (int i = 0; i < KV_TILE && j0 + i < end; ++i) {
+                    const int block = a.tables[(long)b * a.ld_tables + (j0 + i) / a.block_size];
+                    if (block < 0 || block >= a.num_blocks) continue;
+                    const long at = (long)block * a.hk + g;
+                    o = fmaf(sp[i] * a.v_scale[at], (float)a.v_codes[(at * W + tid) * a.block_size + (j0 + i) % a.block_size], o);
+                }
+            }
+            m = mn;
+        }
+        if (tid < a.dk)
+            ((T*)a.out)[(long)t * a.ldo + (long)head * a.ldo_head + tid] = from_f32<T>(l > 0.f ? o / l : l != l ? l : 0.f);
+        if (a.lse && tid == 0) a.lse[(long)t * a.h + head] = l > 0.f ? m + __logf(l) : l != l ? l : -INFINITY;
+    }
+}
+
+extern "C" int64_t athena_kv8_attention_workspace_bytes(int B, int max_rows, int N, int h, int hk, int table_width, int block_size,
+                                                        int dk, int width) {
+    return 0;
+}
+
+extern "C" int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, const int8_t* k_codes, const int8_t* v_codes,
+                                    const float* k_scale, const float* v_scale, int num_blocks, int block_size, int width,
+                                    const int32_t* tables, long ld_tables, int table_width, const int32_t* lens,
+                                    const int32_t* cu_rows, int B, int max_rows, int N, int h, int hk, int dk, int causal,
+                                    float scale, void* out, long ldo, long ldo_head, float* lse, void* workspace,
+                                    int64_t workspace_bytes, athena_stream_t stream) {
+    int rc = kv8_check("athena_kv8_attention", num_blocks, hk, block_size, dk, width);
+    if (rc) return rc;
+    ATHENA_REQUIRE(B > 0 && B <= 65535 && N >= 0 && max_rows > 0 && h > 0 && h <= 65535 && h % hk == 0 && table_width > 0 &&
+                       (long)table_width * block_size < (1L << 31),
+                   ATHENA_E_SHAPE, "athena_kv8_attention: bad shape B=%d N=%d max_rows=%d heads=%d kv_heads=%d table_width=%d", B, N,
+                   max_rows, h, hk, table_width);
+    ATHENA_REQUIRE(dtype == ATHENA_F32 || dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_attention: dtype");
+    if (N == 0) return ATHENA_OK;
+    ATHENA_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && tables && lens && out, ATHENA_E_SHAPE,
+                   "athena_kv8_attention: null operand");
+    ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN,
+                   "athena_kv8_attention: codes must lie on 16 bytes");
+    KvAttn a = {q, ldq, ldq_head, k_codes, v_codes, k_scale, v_scale, tables, ld_tables, lens, cu_rows, out, ldo, ldo_head, lse,
+                table_width, num_blocks, B, N, h, hk, dk, block_size, causal, scale};
+    const dim3 grid(max_rows < 4096 ? max_rows : 4096, h, B), block(KV_TILE);
+    hipStream_t s = (hipStream_t)stream;
+#define KV_SIMPLE(T)                                                                              \
+    do {                                                                                          \
+        if (width == 32) ATHENA_LAUNCH((kv8_attention_kernel<T, 32>), grid, block, 0, s, a);      \
+        else if (width == 64) ATHENA_LAUNCH((kv8_attention_kernel<T, 64>), grid, block, 0, s, a); \
+        else ATHENA_LAUNCH((kv8_attention_kernel<T, 128>), grid, block, 0, s, a);                 \
+    } while (0)
+    if (dtype == ATHENA_BF16) KV_SIMPLE(bf16_t);
+    else KV_SIMPLE(float);
+#undef KV_SIMPLE
+    ATHENA_CHECK_LAUNCH("athena_kv8_attention");
+    return ATHENA_OK;
+}

@@ -3,8 +3,10 @@
 torch is used here for device memory and streams only; every function below enqueues one or
 more kernels of ``libathena_hip.so`` on ``torch.cuda.current_stream()``.
 """
+import collections
 import contextlib
 import ctypes
+import math
 import os
 
 import torch
@@ -1260,3 +1262,199 @@ def axpby(a, x, b, y):
     if x.numel() != y.numel() or x.dtype != y.dtype:
         raise RuntimeError("athena_amd.axpby: operand mismatch")
     _lib.check(_lib.load().athena_axpby(a, _ptr(x), b, _ptr(y), x.numel(), dt(x), _stream()), "athena_axpby")
+
+
+# ------------------------------------------------------------------------------------------ decoding: cache, logits
+KV8_WIDTHS = (32, 64, 128)
+KV8_BLOCKS = (16, 32, 64, 128)
+
+
+def _here(name, *tensors):
+    """Every given tensor lives on the current GPU (kernels go to its current stream)."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise RuntimeError("athena_amd.%s: tensors must live on the current GPU, cuda:%d (got %s)" % (name, here, t.device))
+
+
+def _ints(name, **tensors):
+    """Contiguous int32 tensors of (at least) the given number of elements: name=(tensor, elements)."""
+    for what, (t, n) in tensors.items():
+        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
+            raise RuntimeError("athena_amd.%s: %s must be contiguous int32 of %d elements" % (name, what, n))
+
+
+def _tables(name, tables, B):
+    """(leading dimension, width) of a table of blocks."""
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != B or tables.shape[1] < 1 or \
+            (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise RuntimeError("athena_amd.%s: tables must be int32 [%d, blocks] with rows in one piece" % (name, B))
+    return tables.stride(0), tables.shape[1]
+
+
+def kv8_width(head_size):
+    """Columns that a head of ``head_size`` takes in the 8-bit cache."""
+    for w in KV8_WIDTHS:
+        if head_size <= w:
+            return w
+    raise NotImplementedError("athena_amd: head size %d exceeds the %d columns of the 8-bit cache" % (head_size, KV8_WIDTHS[-1]))
+
+
+KvPlan = collections.namedtuple("KvPlan", ["cu_rows", "slots", "positions", "lens", "free_count", "status"])
+
+
+def kv_plan(lens, new_rows, tables, free_blocks, free_count, block_size, rows, in_place=True):
+    """Blocks and places of the next ``new_rows[b]`` tokens of every request (``new_rows[b]`` < 0: finished, its
+    blocks go back to the stack ``free_blocks[:free_count]``); see ``athena_kv_plan`` in include/athena_hip.h.
+    ``rows``: room for new rows.  ``tables`` and ``free_blocks`` are updated; so are ``lens`` and ``free_count``
+    unless ``in_place`` is false.  Returns a ``KvPlan``; ``status`` (int32 [4]) is not zero where the plan did not
+    fit and nothing was changed."""
+    B = lens.numel()
+    ldt, width = _tables("kv_plan", tables, B)
+    _ints("kv_plan", lens=(lens, 1), new_rows=(new_rows, B), free_blocks=(free_blocks, 1), free_count=(free_count, 1))
+    _here("kv_plan", lens, new_rows, tables, free_blocks, free_count)
+    # one piece of memory for everything the plan writes afresh
+    sizes = (B + 1, rows, rows, 4, 0 if in_place else B, 0 if in_place else 1, 3 * B + 3)
+    cu, slots, positions, status, out, count, work = torch.empty(sum(sizes), dtype=torch.int32, device=lens.device).split(sizes)
+    if in_place:
+        out, count = lens, free_count
+    _lib.check(_lib.load().athena_kv_plan(_ptr(lens), _ptr(new_rows), _ptr(tables), ldt, width, _ptr(free_blocks),
+                                          free_blocks.numel(), _ptr(free_count), B, block_size, rows, cu.data_ptr(),
+                                          slots.data_ptr(), positions.data_ptr(), out.data_ptr(), count.data_ptr(),
+                                          status.data_ptr(), work.data_ptr(), _stream()), "athena_kv_plan")
+    return KvPlan(cu, slots, positions, out, count, status)
+
+
+def _kv8_cache(name, k_codes, v_codes, k_scale, v_scale):
+    """(blocks, kv heads, block size, width) of a cache."""
+    if k_codes.dim() != 4 or v_codes.dim() != 4 or k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or \
+            not k_codes.is_contiguous() or not v_codes.is_contiguous():
+        raise RuntimeError("athena_amd.%s: codes must be contiguous int8 [blocks, heads, tokens, columns] (values: columns, "
+                           "tokens)" % name)
+    nb, hk, bs, w = k_codes.shape
+    if tuple(v_codes.shape) != (nb, hk, w, bs):
+        raise RuntimeError("athena_amd.%s: v_codes must be [%d, %d, %d, %d]" % (name, nb, hk, w, bs))
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float32 or s.numel() != nb * hk or not s.is_contiguous():
+            raise RuntimeError("athena_amd.%s: scales must be contiguous fp32 [%d, %d]" % (name, nb, hk))
+    return nb, hk, bs, w
+
+
+def _head_rows(name, what, x):
+    """(row stride, head stride) of [rows, heads, columns] with contiguous columns."""
+    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise RuntimeError("athena_amd.%s: %s must be [rows, heads, columns] with contiguous columns" % (name, what))
+    return x.stride(0), x.stride(1)
+
+
+def kv8_append(k, v, slots, k_codes, v_codes, k_scale, v_scale):
+    """Keys and values [rows, kv heads, head size] into the 8-bit cache at ``slots`` [rows] (-1 skips a row);
+    see ``athena_kv8_append`` in include/athena_hip.h."""
+    nb, hk, bs, w = _kv8_cache("kv8_append", k_codes, v_codes, k_scale, v_scale)
+    ldk, ldk_h = _head_rows("kv8_append", "k", k)
+    ldv, ldv_h = _head_rows("kv8_append", "v", v)
+    n, heads, dk = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or heads != hk or dk > w:
+        raise RuntimeError("athena_amd.kv8_append: k and v must be alike, [rows, %d, up to %d]" % (hk, w))
+    _ints("kv8_append", slots=(slots, n))
+    _here("kv8_append", k, v, slots, k_codes, v_codes, k_scale, v_scale)
+    _lib.check(_lib.load().athena_kv8_append(_ptr(k), _ptr(v), ldk, ldk_h, ldv, ldv_h, dt(k), _ptr(slots), n, _ptr(k_codes),
+                                             _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), nb, hk, bs, dk, w, _stream()),
+               "athena_kv8_append")
+
+
+def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows=None, max_rows=1, causal=True, scale=None,
+                  out=None, lse=None):
+    """Attention of the query rows [rows, heads, head size] over the 8-bit cache; see ``athena_kv8_attention`` in
+    include/athena_hip.h.  ``cu_rows`` None: row b belongs to sequence b.  ``scale`` None: 1 / sqrt(head size).
+    Rows of ``out`` that belong to no sequence are left as they were (not set, without ``out``)."""
+    nb, hk, bs, w = _kv8_cache("kv8_attention", k_codes, v_codes, k_scale, v_scale)
+    ldq, ldq_h = _head_rows("kv8_attention", "q", q)
+    n, h, dk = q.shape
+    B = lens.numel()
+    ldt, width = _tables("kv8_attention", tables, B)
+    if h % hk or dk > w or dk < 1 or max_rows < 1:
+        raise RuntimeError("athena_amd.kv8_attention: %d heads of %d over %d kv heads of up to %d" % (h, dk, hk, w))
+    if cu_rows is None:
+        if n != B:
+            raise RuntimeError("athena_amd.kv8_attention: %d rows for %d sequences need cu_rows" % (n, B))
+        max_rows = 1
+        _ints("kv8_attention", lens=(lens, 1))
+    else:
+        _ints("kv8_attention", lens=(lens, 1), cu_rows=(cu_rows, B + 1))
+    if out is None:
+        out = torch.empty((n, h, dk), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise RuntimeError("athena_amd.kv8_attention: out must be like q")
+    ldo, ldo_h = _head_rows("kv8_attention", "out", out)
+    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n * h or not lse.is_contiguous()):
+        raise RuntimeError("athena_amd.kv8_attention: lse must be contiguous fp32 [%d, %d]" % (n, h))
+    _here("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows, out, lse)
+    lib = _lib.load()
+    need = lib.athena_kv8_attention_workspace_bytes(B, max_rows, n, h, hk, width, bs, dk, w)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.check(lib.athena_kv8_attention(_ptr(q), ldq, ldq_h, dt(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale),
+                                        nb, bs, w, _ptr(tables), ldt, width, _ptr(lens), _ptr(cu_rows), B, max_rows, n, h, hk,
+                                        dk, 1 if causal else 0, scale if scale is not None else 1.0 / math.sqrt(dk),
+                                        out.data_ptr(), ldo, ldo_h, _ptr(lse), _ptr(ws), need, _stream()),
+               "athena_kv8_attention")
+    return out
+
+
+def _row_vector(name, what, t, rows):
+    if t is not None and (t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous()):
+        raise RuntimeError("athena_amd.%s: %s must be contiguous fp32 [%d]" % (name, what, rows))
+
+
+def _row_matrix(name, what, t, dtype, rows, cols):
+    """Leading dimension of [rows, cols], or 0 for one row [cols] / [1, cols] that serves all."""
+    if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] != cols or (cols > 1 and t.stride(-1) != 1) or \
+            (t.dim() == 2 and t.shape[0] not in (1, rows)):
+        raise RuntimeError("athena_amd.%s: %s must be %s [%d, %d] or one such row" % (name, what, dtype, rows, cols))
+    return t.stride(0) if t.dim() == 2 and t.shape[0] == rows else 0
+
+
+def logits_process(logits, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
+                   bias_ids=None, bias_values=None, allowed=None, out=None):
+    """Penalties for repeated tokens, biases and a grammar mask on logits [rows, classes]; see
+    ``athena_logits_process`` in include/athena_hip.h.  ``history`` int32 [rows, L] with ``history_len`` int32
+    [rows]; ``repetition``, ``presence``, ``frequency`` fp32 [rows]; ``bias`` fp32 [rows or 1, classes];
+    ``bias_ids`` / ``bias_values`` int32 / fp32 [rows, n]; ``allowed`` int32 [rows or 1, ceil(classes / 32)], a bit per
+    class.  Returns ``out`` (a new tensor unless given; it may be ``logits``)."""
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError("athena_amd.logits_process: logits must be [rows, classes] with contiguous rows")
+    R, V = logits.shape
+    L = ldh = ldb = ldi = ldv = lda = nb = 0
+    if history is not None:
+        L = history.shape[-1]
+        if history.dim() != 2 or history.shape[0] != R:
+            raise RuntimeError("athena_amd.logits_process: history must be int32 [%d, tokens]" % R)
+        ldh = _row_matrix("logits_process", "history", history, torch.int32, R, L)
+        if history_len is not None:
+            _ints("logits_process", history_len=(history_len, R))
+    elif history_len is not None or repetition is not None or presence is not None or frequency is not None:
+        raise RuntimeError("athena_amd.logits_process: penalties need a history")
+    _row_vector("logits_process", "repetition", repetition, R)
+    _row_vector("logits_process", "presence", presence, R)
+    _row_vector("logits_process", "frequency", frequency, R)
+    if bias is not None:
+        ldb = _row_matrix("logits_process", "bias", bias, torch.float32, R, V)
+    if (bias_ids is None) != (bias_values is None):
+        raise RuntimeError("athena_amd.logits_process: bias_ids and bias_values come together")
+    if bias_ids is not None:
+        nb = bias_ids.shape[-1]
+        ldi = _row_matrix("logits_process", "bias_ids", bias_ids, torch.int32, R, nb)
+        ldv = _row_matrix("logits_process", "bias_values", bias_values, torch.float32, R, nb)
+    if allowed is not None:
+        lda = _row_matrix("logits_process", "allowed", allowed, torch.int32, R, (V + 31) // 32)
+    if out is None:
+        out = torch.empty((R, V), dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1):
+        raise RuntimeError("athena_amd.logits_process: out must be like logits")
+    _here("logits_process", logits, history, history_len, repetition, presence, frequency, bias, bias_ids, bias_values, allowed,
+          out)
+    _lib.check(_lib.load().athena_logits_process(
+        _ptr(logits), logits.stride(0) if R > 1 else V, dt(logits), R, V, _ptr(history), ldh, L, _ptr(history_len), _ptr(repetition),
+        _ptr(presence), _ptr(frequency), _ptr(bias), ldb, _ptr(bias_ids), ldi, _ptr(bias_values), ldv, nb, _ptr(allowed), lda,
+        out.data_ptr(), out.stride(0) if R > 1 else V, _stream()), "athena_logits_process")
+    return out

@@ -746,6 +746,81 @@ int athena_axpby(float a, const void* x, float b, void* y, long n, int dtype, at
 #define ATHENA_COPY_MANY_MAX 8
 int athena_copy_many(const void* const* src, void* const* dst, const long* bytes, int n, athena_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged key / value cache in 8 bits, for decoding.  The reference runs its decoder over the whole
+ * history at every step (SpeechTransformer.time_propagate, athena/models/speech_transformer.py:164-194)
+ * and keeps nothing; these entry points let a step compute its newest rows only.
+ *
+ * The cache of one attention layer, ``num_blocks`` blocks of ``block_size`` (16, 32, 64 or 128) tokens:
+ *   k_codes int8 [num_blocks][hk][block_size][width]   k_scale fp32 [num_blocks][hk]
+ *   v_codes int8 [num_blocks][hk][width][block_size]   v_scale fp32 [num_blocks][hk]
+ * An element stands for code * scale.  width is 32, 64 or 128; heads of dk <= width columns use the first
+ * dk, the others hold zeros.  Codes start on 16 bytes.  Place p of the cache is token p % block_size of block
+ * p / block_size; num_blocks * block_size < 2^31.
+ *
+ * athena_kv_plan: the blocks and places of the next new_rows[b] tokens of every request.  lens[b] tokens are
+ * cached already, in the blocks tables[b * ld_tables + 0 ...] (table_width entries a request);
+ * free_blocks[0 .. free_count[0]) is a stack of free blocks.  new_rows[b] < 0 marks a finished request: its
+ * blocks are put on top of the stack (in request and table order) before any are taken, and its length
+ * becomes 0.  Entries beyond those lens needs are filled from the top of the stack, in request order.
+ * Written: cu_rows [B + 1] (rows of the requests one behind the other; request b has rows
+ * cu_rows[b] .. cu_rows[b + 1]), slots [rows] (the place of each row; -1 behind the last row), positions
+ * [rows] (a row's index in its sequence; 0 behind the last row), the new table entries, the returned blocks,
+ * lens_out [B] and free_count_out [1] (each may be the input itself), and status [4]: {blocks missing,
+ * requests with a negative length or longer than their table, rows missing, returned blocks beyond
+ * free_capacity}.  A plan that does not fit leaves a status that is not zero and changes nothing: no rows
+ * (cu_rows 0, slots -1), lens_out = lens, free_count_out = free_count.  ``work``: int32 [3 * B + 3].
+ * A block belongs to one request. */
+int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int32_t* tables, long ld_tables, int table_width,
+                   int32_t* free_blocks, int free_capacity, const int32_t* free_count, int B, int block_size, int rows,
+                   int32_t* cu_rows, int32_t* slots, int32_t* positions, int32_t* lens_out, int32_t* free_count_out,
+                   int32_t* status, int32_t* work, athena_stream_t stream);
+
+/* Keys and values of N rows into their places.  Row t: k[t * ldk + head * ldk_head + c], c < dk; a slot
+ * outside [0, num_blocks * block_size) skips its row.  Rows of one block stand one behind the other (as
+ * athena_kv_plan lays them out), and no place comes twice.  The scale of a block and head is the largest
+ * magnitude written so far / 127: it only grows, and the codes in front of the new ones are then brought to
+ * the grown scale (round half to even of code * old / new); a run that begins at a block's first place
+ * begins the block again, whatever its scale was.  Codes are round half to even of x / scale.  A value that
+ * is not finite makes its block's scale not finite: the block then stands for NaN until it is begun again. */
+int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, long ldv, long ldv_head, int dtype,
+                      const int32_t* slots, int N, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
+                      int num_blocks, int hk, int block_size, int dk, int width, athena_stream_t stream);
+
+/* Attention over the cache: out[t, head] = sum_j softmax_j(scale * q[t, head] . k_j) v_j over the cached
+ * tokens of t's sequence.  Sequence b has lens[b] tokens (its new ones included) and the query rows
+ * cu_rows[b] .. cu_rows[b + 1] of q, its last tokens; cu_rows null: one row per sequence.  causal: row i of
+ * n sees the tokens j <= lens[b] - n + i.  Query head i reads kv head i / (h / hk).  A row that sees nothing
+ * gives zeros (lse -inf).  Table entries outside [0, num_blocks) hold no tokens; lengths are cut at
+ * table_width * block_size, rows at N; rows that belong to no sequence are left as they were.
+ * max_rows: the largest number of rows of a sequence (it shapes the launch; results do not depend on it).
+ * lse: fp32 [N][h], natural logarithm of the sum of exponentials, or null.
+ * ld_tables may be 0: every sequence then reads the same blocks.
+ * ``workspace``: athena_kv8_attention_workspace_bytes (0: none is needed). */
+int64_t athena_kv8_attention_workspace_bytes(int B, int max_rows, int N, int h, int hk, int table_width, int block_size,
+                                             int dk, int width);
+int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, const int8_t* k_codes, const int8_t* v_codes,
+                         const float* k_scale, const float* v_scale, int num_blocks, int block_size, int width,
+                         const int32_t* tables, long ld_tables, int table_width, const int32_t* lens,
+                         const int32_t* cu_rows, int B, int max_rows, int N, int h, int hk, int dk, int causal,
+                         float scale, void* out, long ldo, long ldo_head, float* lse, void* workspace,
+                         int64_t workspace_bytes, athena_stream_t stream);
+
+/* Penalties, biases and a grammar mask on the logits of a decoding step, between the output layer and the
+ * search (the reference adds scorers to log-probabilities on the host, athena/tools/beam_search.py:120-150).
+ * With c = occurrences of class v in history[r, 0 .. history_len[r]) (history_len null: L; ids outside
+ * [0, V) count nowhere):
+ *   x = logit;  c > 0: x = x > 0 ? x / repetition[r] : x * repetition[r];  x -= frequency[r] c + presence[r];
+ *   x += bias[r * ld_bias + v] + sum of bias_values[r, j] over bias_ids[r, j] == v;
+ *   -inf unless bit v % 32 of word v / 32 of allowed[r * ld_allowed + ...] is set.
+ * Any of history, repetition, presence, frequency, bias, bias_ids (nb = 0), allowed may be null.  ld_bias and
+ * ld_allowed may be 0 (one row for all).  out has the type of the logits and may be the logits. */
+int athena_logits_process(const void* logits, long ldl, int dtype, int R, int V, const int32_t* history, long ld_history,
+                          int L, const int32_t* history_len, const float* repetition, const float* presence,
+                          const float* frequency, const float* bias, long ld_bias, const int32_t* bias_ids,
+                          long ld_bias_ids, const float* bias_values, long ld_bias_values, int nb,
+                          const int32_t* allowed, long ld_allowed, void* out, long ldo, athena_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
