@@ -201,15 +201,18 @@ extern "C" int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int3
 }
 
 // ---------------------------------------------------------------- writing new keys and values
-// A run of consecutive rows that go to the same block is one unit of work: the block's scale grows to the
-// largest magnitude of the run / 127 (from nothing where the run begins the block), codes already in the
-// block in front of the run are brought to a grown scale, and the run's codes are written.  One wave per
-// (run, kv head, keys or values); waves of one block never meet, as a run is taken by the wave that finds
-// its first row.
+// Consecutive rows that go to the same block are one run: the block's scale grows to the largest magnitude of
+// the run / 127 (from nothing where the run begins the block), codes in front of the run are brought to a grown
+// scale, and the run's codes are written.  One wave per (run, kv head, keys or values); the wave that finds a
+// run's first row takes all of it, so waves of one block never meet.
 //
 // Codes are round-half-to-even(x / scale) exactly: the product with the reciprocal in fp32 is off by less
 // than 127 * 2^-23, so a quotient within 1e-4 of a border is divided again in 64 bits, where quotients of
 // fp32 operands of this size cannot come closer than 2^-34 to a border without lying on it.
+//
+// A lane holds two columns of 16 consecutive places, so that the values' codes (16 bytes of one column) leave
+// in one store.  Bound by the rows' way in and the codes' way out; a run of more places than the wave holds at
+// once reads its rows twice, the second time from the caches.
 template <typename T> struct AppendSide {
     const T* x;
     long ld_row, ld_head;
@@ -221,7 +224,7 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
     const float f = x * inv;
     float q = rintf(f);
     if (fabsf(fabsf(f - q) - 0.5f) < 1e-4f || s < 1e-30f) q = s > 0.f ? (float)rint((double)x / (double)s) : 0.f;
-    return (int)fminf(fmaxf(q, -127.f), 127.f);             // (NaN: -127 or 127; the scale is NaN then)
+    return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
 __device__ __forceinline__ int recode(int q, float s0, float s1, float ratio) {
     const float f = (float)q * ratio;
@@ -229,72 +232,174 @@ __device__ __forceinline__ int recode(int q, float s0, float s1, float ratio) {
     if (fabsf(fabsf(f - r) - 0.5f) < 1e-4f || s0 < 1e-30f) r = (float)rint((double)q * (double)s0 / (double)s1);
     return (int)r;
 }
-
-template <typename T>
-__global__ __launch_bounds__(256) void kv8_append_kernel(AppendSide<T> ks, AppendSide<T> vs, const int32_t* __restrict__ slots,
-                                                         int N, int rows_per_wg, int hk, int dk, int width, int block_size,
-                                                         long slots_end) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, head = blockIdx.y;
-    const int t0 = blockIdx.x * rows_per_wg;
-    // first rows of runs among the workgroup's rows
-    bool leads = false;
-    if (lane < rows_per_wg && t0 + lane < N) {
-        const int s = slots[t0 + lane], p = t0 + lane > 0 ? slots[t0 + lane - 1] : -1;
-        leads = s >= 0 && s < slots_end && !(p >= 0 && p < slots_end && p / block_size == s / block_size);
+// the first ``keep`` of four codes in a word
+__device__ __forceinline__ unsigned recode4(unsigned w, int keep, float s0, float s1, float ratio) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned q = (unsigned)recode((int8_t)(w >> (8 * i)), s0, s1, ratio) & 0xffu;
+        if (i < keep) w = (w & ~(0xffu << (8 * i))) | (q << (8 * i));
     }
-    unsigned long long found = __ballot(leads);
-    int job = 0;
-    while (found) {
-        const int t = t0 + __ffsll((long long)found) - 1;
-        found &= found - 1;
-#pragma unroll 1
-        for (int side = 0; side < 2; ++side, ++job) {
-            if (job % nw != w) continue;
-            const AppendSide<T> a = side ? vs : ks;
-            const int block = slots[t] / block_size;
-            // the run's length and first place
-            int n = 0, place = block_size;
-            for (;; n += 64) {
-                const int s = t + n + lane < N ? slots[t + n + lane] : -1;
-                const bool in = s >= 0 && s < slots_end && s / block_size == block;
-                const unsigned long long same = __ballot(in);
-                const int len = same == ~0ull ? 64 : __ffsll((long long)~same) - 1;
-                int p = lane < len ? s % block_size : block_size;
+    return w;
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void append_run(const AppendSide<T>& a, bool values, const int32_t* __restrict__ slots, long slots_end,
+                                           int t, int n, int first, bool straight, int block, int head, int hk, int dk,
+                                           int block_size, bool pairs, int lane) {
+    constexpr int LR = W / 2, SUB = 64 / LR;                // lanes of a row, groups of 16 places side by side
+    const int sub = lane / LR, c = 2 * (lane % LR);
+    const T* x = a.x + (long)t * a.ld_row + (long)head * a.ld_head;
+    const long at = (long)block * hk + head;
+    int8_t* codes = a.codes + at * W * block_size;
+    const int step = 16 * SUB, begin = first & ~15, end = first + n;
+    float v[16][2];
+    auto load = [&](int base) {                             // the two columns of places base + 16 sub ...
+        const int p0 = base + 16 * sub;
 #pragma unroll
-                for (int o = 32; o > 0; o >>= 1) p = min(p, __shfl_xor(p, o, 64));
-                place = min(place, p);
-                if (len < 64) { n += len; break; }
-            }
-            const T* x = a.x + (long)t * a.ld_row + (long)head * a.ld_head;
-            unsigned top = 0;                   // largest magnitude, as bits: NaN over infinity over numbers
-            for (int e = lane; e < n * dk; e += 64) {
-                const int r = e / dk, c = e - r * dk;
-                top = max(top, __float_as_uint(to_f32<T>(x[(long)r * a.ld_row + c])) & 0x7fffffffu);
-            }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-            const long at = (long)block * hk + head;
-            const float s0 = place == 0 ? 0.f : a.scale[at], s1n = __uint_as_float(top) / 127.f;
-            // (as whole numbers, so that a scale that is NaN stays)
-            const float s1 = __uint_as_float(max(__float_as_uint(s0) & 0x7fffffffu, __float_as_uint(s1n) & 0x7fffffffu));
-            int8_t* codes = a.codes + at * (long)width * block_size;
-            const int row = side ? 1 : width, col = side ? block_size : 1;      // steps of a token / a column
-            if (s1 > s0 && place > 0) {
-                const float ratio = s0 / s1;
-                for (int e = lane; e < place * width; e += 64) {
-                    const int r = e / width, c = e - r * width;
-                    int8_t* p = codes + (long)r * row + (long)c * col;
-                    *p = (int8_t)recode(*p, s0, s1, ratio);
+        for (int i = 0; i < 16; ++i) {
+            v[i][0] = v[i][1] = 0.f;
+            if (p0 + i >= first && p0 + i < end && c < dk) {
+                const T* p = x + (long)(p0 + i - first) * a.ld_row + c;
+                if (pairs && c + 1 < dk) {
+                    struct alignas(2 * sizeof(T)) Pair { T e[2]; };
+                    const Pair two = *(const Pair*)p;
+                    v[i][0] = to_f32<T>(two.e[0]);
+                    v[i][1] = to_f32<T>(two.e[1]);
+                } else {
+                    v[i][0] = to_f32<T>(p[0]);
+                    if (c + 1 < dk) v[i][1] = to_f32<T>(p[1]);
                 }
             }
-            const float inv = s1 > 0.f ? 1.f / s1 : 0.f;
-            for (int e = lane; e < n * width; e += 64) {
-                const int r = e / width, c = e - r * width;
-                const int off = slots[t + r] % block_size;
-                const float v = c < dk ? to_f32<T>(x[(long)r * a.ld_row + c]) : 0.f;
-                codes[(long)off * row + (long)c * col] = (int8_t)code_of(v, s1, inv);
+        }
+    };
+    unsigned top = 0;                                       // largest magnitude, as bits: NaN over infinity over numbers
+    const auto mag = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
+    if (straight) {
+        for (int base = begin; base < end; base += step) {
+            load(base);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, max(mag(v[i][0]), mag(v[i][1])));
+        }
+    } else {
+        for (int e = lane; e < n * dk; e += 64) {
+            const int r = e / dk, s = slots[t + r];
+            if (s >= 0 && s < slots_end) top = max(top, mag(to_f32<T>(x[(long)r * a.ld_row + (e - r * dk)])));
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
+    const float s0 = first == 0 ? 0.f : a.scale[at];
+    // (as whole numbers, so that a scale that is not finite stays; it is kept as NaN)
+    const unsigned bits = max(mag(s0), mag(__uint_as_float(top) / 127.f));
+    const float s1 = __uint_as_float(bits < 0x7f800000u ? bits : 0x7fc00000u);
+    if (s1 > s0 && first > 0) {
+        const float ratio = s0 / s1;
+        const int words = values ? (first + 15) / 16 : first * W / 16, columns = values ? W : 1;
+        for (int e = lane; e < words * columns; e += 64) {
+            const int col = e / words, k = e - col * words;
+            uint4* p = (uint4*)(codes + (values ? col * block_size : 0) + 16 * k);
+            const int keep = values ? first - 16 * k : 16;
+            uint4 w = *p;
+            w.x = recode4(w.x, keep, s0, s1, ratio);
+            w.y = recode4(w.y, keep - 4, s0, s1, ratio);
+            w.z = recode4(w.z, keep - 8, s0, s1, ratio);
+            w.w = recode4(w.w, keep - 12, s0, s1, ratio);
+            *p = w;
+        }
+    }
+    const float inv = s1 > 0.f ? 1.f / s1 : 0.f;
+    if (straight) {
+        for (int base = begin; base < end; base += step) {
+            if (end - begin > step) load(base);             // (otherwise the registers hold the rows still)
+            const int p0 = base + 16 * sub;
+            if (values) {
+                if (p0 >= first && p0 + 16 <= end) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        unsigned w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = 0;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) w[i] |= ((unsigned)code_of(v[4 * i + r][k], s1, inv) & 0xffu) << (8 * r);
+                        }
+                        *(uint4*)(codes + (c + k) * block_size + p0) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (p0 + i >= first && p0 + i < end) {
+                            codes[c * block_size + p0 + i] = (int8_t)code_of(v[i][0], s1, inv);
+                            codes[(c + 1) * block_size + p0 + i] = (int8_t)code_of(v[i][1], s1, inv);
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (p0 + i >= first && p0 + i < end) {
+                        const unsigned two = ((unsigned)code_of(v[i][0], s1, inv) & 0xffu) | ((unsigned)code_of(v[i][1], s1, inv) & 0xffu) << 8;
+                        *(uint16_t*)(codes + (p0 + i) * W + c) = (uint16_t)two;
+                    }
             }
-            if (lane == 0) a.scale[at] = s1;
+        }
+    } else {
+        for (int r = 0; r < n; ++r) {                       // in the rows' order: of two rows for one place the later stays
+            const int s = slots[t + r];
+            if (s < 0 || s >= slots_end) continue;
+            for (int col = lane; col < W; col += 64) {
+                const float f = col < dk ? to_f32<T>(x[(long)r * a.ld_row + col]) : 0.f;
+                codes[values ? col * block_size + s % block_size : (s % block_size) * W + col] = (int8_t)code_of(f, s1, inv);
+            }
+        }
+    }
+    if (lane == 0) a.scale[at] = s1;
+}
+
+template <typename T, int W>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendSide<T> ks, AppendSide<T> vs, const int32_t* __restrict__ slots,
+                                                         int N, int rows_per_wg, int hk, int dk, int block_size, int k_pairs,
+                                                         int v_pairs, long slots_end) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, head = blockIdx.y;
+    const int t0 = blockIdx.x * rows_per_wg;
+    const auto good = [&](int s) { return s >= 0 && s < slots_end; };
+    // first rows of runs among the workgroup's rows; skipped rows do not end a run
+    bool leads = false;
+    if (lane < rows_per_wg && t0 + lane < N) {
+        const int s = slots[t0 + lane];
+        if (good(s)) {
+            int p = t0 + lane - 1;
+            while (p >= 0 && !good(slots[p])) --p;
+            leads = p < 0 || slots[p] / block_size != s / block_size;
+        }
+    }
+    unsigned long long found = __ballot(leads);
+    for (int job = 0; found; job += 2) {
+        const int t = t0 + __ffsll((long long)found) - 1;
+        found &= found - 1;
+        // both sides of a run go to neighbouring waves
+        for (int side = 0; side < 2; ++side) {
+            if ((job + side) % nw != w) continue;
+            const int s0 = slots[t], block = s0 / block_size;
+            int n = 0, first = block_size;                  // rows up to the run's last one, first place
+            bool straight = true, more = true;              // straight: no row skipped, places in order
+            for (int r0 = 0; more; r0 += 64) {
+                const int r = r0 + lane, s = t + r < N ? slots[t + r] : -1;
+                const unsigned long long mine = __ballot(good(s) && s / block_size == block),
+                                         other = __ballot(t + r >= N || (good(s) && s / block_size != block));
+                const unsigned long long in = other ? mine & ((other & -other) - 1) : mine;
+                more = !other;
+                if (in) {
+                    const int last = 63 - __clzll((long long)in);
+                    straight = straight && n == r0 && __ballot(lane <= last && s != s0 + r) == 0;
+                    n = r0 + last + 1;
+                    int p = (in >> lane) & 1 ? s % block_size : block_size;
+#pragma unroll
+                    for (int o = 32; o > 0; o >>= 1) p = min(p, __shfl_xor(p, o, 64));
+                    first = min(first, p);
+                }
+            }
+            if (side) append_run<T, W>(vs, true, slots, slots_end, t, n, first, straight, block, head, hk, dk, block_size, v_pairs, lane);
+            else append_run<T, W>(ks, false, slots, slots_end, t, n, first, straight, block, head, hk, dk, block_size, k_pairs, lane);
         }
     }
 }
@@ -323,13 +428,25 @@ extern "C" int athena_kv8_append(const void* k, const void* v, long ldk, long ld
     const int per = (long)N * hk <= 4096 ? 1 : 16;
     const dim3 grid((N + per - 1) / per, hk), block(per == 1 ? 128 : 256);
     const long end = (long)num_blocks * block_size;
-    if (dtype == ATHENA_BF16) {
-        AppendSide<bf16_t> ks = {(const bf16_t*)k, ldk, ldk_head, k_codes, k_scale}, vs = {(const bf16_t*)v, ldv, ldv_head, v_codes, v_scale};
-        ATHENA_LAUNCH(kv8_append_kernel<bf16_t>, grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, width, block_size, end);
-    } else {
-        AppendSide<float> ks = {(const float*)k, ldk, ldk_head, k_codes, k_scale}, vs = {(const float*)v, ldv, ldv_head, v_codes, v_scale};
-        ATHENA_LAUNCH(kv8_append_kernel<float>, grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, width, block_size, end);
-    }
+    const size_t two = dtype == ATHENA_BF16 ? 4 : 8;        // two elements in one load where rows and heads begin on them
+    const int kp = (uintptr_t)k % two == 0 && ldk % 2 == 0 && ldk_head % 2 == 0;
+    const int vp = (uintptr_t)v % two == 0 && ldv % 2 == 0 && ldv_head % 2 == 0;
+#define KV_APPEND(T, W)                                                                                                     \
+    do {                                                                                                                    \
+        AppendSide<T> ks = {(const T*)k, ldk, ldk_head, k_codes, k_scale}, vs = {(const T*)v, ldv, ldv_head, v_codes, v_scale}; \
+        ATHENA_LAUNCH((kv8_append_kernel<T, W>), grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, block_size, \
+                      kp, vp, end);                                                                                         \
+    } while (0)
+#define KV_APPEND_W(T)                     \
+    do {                                   \
+        if (width == 32) KV_APPEND(T, 32); \
+        else if (width == 64) KV_APPEND(T, 64); \
+        else KV_APPEND(T, 128);            \
+    } while (0)
+    if (dtype == ATHENA_BF16) KV_APPEND_W(bf16_t);
+    else KV_APPEND_W(float);
+#undef KV_APPEND_W
+#undef KV_APPEND
     ATHENA_CHECK_LAUNCH("athena_kv8_append");
     return ATHENA_OK;
 }

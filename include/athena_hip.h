@@ -778,11 +778,12 @@ int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int32_t* tables
 
 /* Keys and values of N rows into their places.  Row t: k[t * ldk + head * ldk_head + c], c < dk; a slot
  * outside [0, num_blocks * block_size) skips its row.  Rows of one block stand one behind the other (as
- * athena_kv_plan lays them out), and no place comes twice.  The scale of a block and head is the largest
+ * athena_kv_plan lays them out; skipped rows may stand between them); of two rows for one place the later
+ * stays.  The scale of a block and head is the largest
  * magnitude written so far / 127: it only grows, and the codes in front of the new ones are then brought to
  * the grown scale (round half to even of code * old / new); a run that begins at a block's first place
  * begins the block again, whatever its scale was.  Codes are round half to even of x / scale.  A value that
- * is not finite makes its block's scale not finite: the block then stands for NaN until it is begun again. */
+ * is not finite makes its block's scale NaN: the block then stands for NaN until it is begun again. */
 int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, long ldv, long ldv_head, int dtype,
                       const int32_t* slots, int N, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
                       int num_blocks, int hk, int block_size, int dk, int width, athena_stream_t stream);

@@ -1,0 +1,142 @@
+"""What the decoding operators refuse, checked in front of any launch (no GPU is needed), and the loop
+restatements the GPU tests compare with, checked against hand-made cases."""
+import ctypes
+
+import pytest
+import torch
+
+from athena_amd import _lib, ops
+from oracle import kv_cache as ok
+
+
+def _cache(nb=4, hk=2, bs=16, w=32):
+    return (torch.zeros(nb, hk, bs, w, dtype=torch.int8), torch.zeros(nb, hk, w, bs, dtype=torch.int8), torch.zeros(nb, hk),
+            torch.zeros(nb, hk))
+
+
+def _i(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("change", ["codes_type", "codes_shape", "codes_strided", "scale_size", "scale_type", "heads", "head_size",
+                                    "k_v_differ", "slots_type", "slots_short", "k_columns_strided"])
+def test_append_refusals(change):
+    kc, vc, ks, vs = _cache()
+    k, v, slots = torch.zeros(3, 2, 24), torch.zeros(3, 2, 24), _i(3)
+    if change == "codes_type": kc = kc.to(torch.uint8)
+    if change == "codes_shape": vc = vc.transpose(2, 3).contiguous()
+    if change == "codes_strided": kc = kc.transpose(0, 1)
+    if change == "scale_size": ks = torch.zeros(4)
+    if change == "scale_type": vs = vs.double()
+    if change == "heads": k, v = torch.zeros(3, 3, 24), torch.zeros(3, 3, 24)
+    if change == "head_size": k, v = torch.zeros(3, 2, 33), torch.zeros(3, 2, 33)
+    if change == "k_v_differ": v = v.to(torch.bfloat16)
+    if change == "slots_type": slots = slots.long()
+    if change == "slots_short": slots = _i(2)
+    if change == "k_columns_strided": k = torch.zeros(3, 2, 48)[..., ::2]
+    with pytest.raises(RuntimeError, match="kv8_append"):
+        ops.kv8_append(k, v, slots, kc, vc, ks, vs)
+
+
+@pytest.mark.parametrize("change", ["heads", "head_size", "rows_without_cu", "cu_short", "tables_type", "tables_rows", "tables_strided",
+                                    "lens_type", "out_shape", "out_type", "lse", "max_rows"])
+def test_attention_refusals(change):
+    kc, vc, ks, vs = _cache()
+    q, tables, lens, kw = torch.zeros(3, 4, 32), _i(3, 2), _i(3), {}
+    if change == "heads": q = torch.zeros(3, 3, 32)
+    if change == "head_size": q = torch.zeros(3, 4, 33)
+    if change == "rows_without_cu": q = torch.zeros(4, 4, 32)
+    if change == "cu_short": kw = dict(cu_rows=_i(3))
+    if change == "tables_type": tables = tables.long()
+    if change == "tables_rows": tables = _i(2, 2)
+    if change == "tables_strided": tables = _i(3, 4)[:, ::2]
+    if change == "lens_type": lens = lens.long()
+    if change == "out_shape": kw = dict(out=torch.zeros(3, 4, 16))
+    if change == "out_type": kw = dict(out=torch.zeros(3, 4, 32, dtype=torch.bfloat16))
+    if change == "lse": kw = dict(lse=torch.zeros(3, 4).double())
+    if change == "max_rows": kw = dict(cu_rows=_i(4), max_rows=0)
+    with pytest.raises(RuntimeError, match="kv8_attention"):
+        ops.kv8_attention(q, kc, vc, ks, vs, tables, lens, **kw)
+
+
+@pytest.mark.parametrize("change", ["lens_type", "new_short", "tables_rows", "free_type", "count_type"])
+def test_plan_refusals(change):
+    lens, new, tables, free, count = _i(3), _i(3), _i(3, 4), _i(8), _i(1)
+    if change == "lens_type": lens = lens.long()
+    if change == "new_short": new = _i(2)
+    if change == "tables_rows": tables = _i(2, 4)
+    if change == "free_type": free = free.float()
+    if change == "count_type": count = count.long()
+    with pytest.raises(RuntimeError, match="kv_plan"):
+        ops.kv_plan(lens, new, tables, free, count, 16, 8)
+
+
+@pytest.mark.parametrize("change", ["logits_dim", "logits_strided", "history_rows", "history_type", "len_type", "no_history", "repetition",
+                                    "bias", "ids_alone", "allowed", "allowed_type", "out"])
+def test_logits_refusals(change):
+    x, kw = torch.zeros(2, 40), dict(history=_i(2, 5))
+    if change == "logits_dim": x = torch.zeros(40)
+    if change == "logits_strided": x = torch.zeros(2, 80)[:, ::2]
+    if change == "history_rows": kw = dict(history=_i(3, 5))
+    if change == "history_type": kw = dict(history=torch.zeros(2, 5))
+    if change == "len_type": kw["history_len"] = torch.zeros(2, dtype=torch.int64)
+    if change == "no_history": kw = dict(presence=torch.zeros(2))
+    if change == "repetition": kw["repetition"] = torch.ones(3)
+    if change == "bias": kw = dict(bias=torch.zeros(2, 39))
+    if change == "ids_alone": kw = dict(bias_ids=_i(2, 1))
+    if change == "allowed": kw = dict(allowed=_i(2, 1))
+    if change == "allowed_type": kw = dict(allowed=torch.zeros(2, 2, dtype=torch.int64))
+    if change == "out": kw["out"] = torch.zeros(2, 40, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="logits_process"):
+        ops.logits_process(x, **kw)
+
+
+def test_the_c_entries_refuse_before_any_launch():
+    lib, p = _lib.load(), ctypes.c_void_p(4096)         # an address that is never followed
+    attn = lambda bs=16, w=32, h=4, dk=32, dtype=0, q=p, nb=4, B=1, mr=1, codes=p: lib.athena_kv8_attention(
+        q, 128, 32, dtype, codes, p, p, p, nb, bs, w, p, 1, 1, p, None, B, mr, 1, h, 2, dk, 1, 1.0, p, 128, 32, None, None, 0, None)
+    for kw in (dict(bs=24), dict(w=48), dict(h=3), dict(dk=33), dict(dk=0), dict(dtype=2), dict(q=None), dict(nb=0), dict(B=0),
+               dict(B=70000), dict(mr=0), dict(nb=1 << 28), dict(codes=ctypes.c_void_p(4100))):
+        assert attn(**kw) < 0, kw
+        assert b"athena_kv8_attention" in lib.athena_last_error()
+    append = lambda bs=16, w=32, dk=32, dtype=0, k=p, n=1, codes=p: lib.athena_kv8_append(
+        k, p, 64, 32, 64, 32, dtype, p, n, codes, p, p, p, 4, 2, bs, dk, w, None)
+    for kw in (dict(bs=8), dict(w=256), dict(dk=64), dict(dtype=5), dict(k=None), dict(n=-1), dict(codes=ctypes.c_void_p(4097))):
+        assert append(**kw) < 0, kw
+        assert b"athena_kv8_append" in lib.athena_last_error()
+    plan = lambda B=1, W=4, ld=4, free=4, bs=16, rows=1, lens=p: lib.athena_kv_plan(
+        lens, p, p, ld, W, p, free, p, B, bs, rows, p, p, p, p, p, p, p, None)
+    for kw in (dict(B=0), dict(W=0), dict(ld=3), dict(free=0), dict(bs=20), dict(rows=-1), dict(lens=None), dict(W=1 << 27, ld=1 << 27)):
+        assert plan(**kw) < 0, kw
+        assert b"athena_kv_plan" in lib.athena_last_error()
+    logits = lambda R=1, V=40, ldl=40, dtype=0, x=p, nb=0: lib.athena_logits_process(
+        x, ldl, dtype, R, V, None, 0, 0, None, None, None, None, None, 0, None, 0, None, 0, nb, None, 0, p, 40, None)
+    for kw in (dict(R=-1), dict(V=0), dict(ldl=39), dict(dtype=3), dict(x=None), dict(nb=1), dict(R=70000)):
+        assert logits(**kw) < 0, kw
+        assert b"athena_logits_process" in lib.athena_last_error()
+    assert logits(R=0) == 0 and append(n=0) == 0
+
+
+def test_cache_width():
+    assert [ops.kv8_width(n) for n in (1, 32, 33, 64, 65, 128)] == [32, 32, 64, 64, 128, 128]
+    with pytest.raises(NotImplementedError):
+        ops.kv8_width(129)
+
+
+def test_oracle_plan_takes_and_gives_back():
+    got = ok.plan([16, 5, 33], [1, -1, 0], [[3, -1, -1], [7, -1, -1], [1, 2, 4]], [9, -1, -1], 1, 16, 4)
+    # request 1's block 7 goes on top of the stack and request 0 takes it at once
+    assert got["cu_rows"] == [0, 1, 1, 1] and got["slots"] == [7 * 16, -1, -1, -1] and got["positions"] == [16, 0, 0, 0]
+    assert got["lens"] == [17, 0, 33] and got["free_count"] == 1 and got["tables"][0] == [3, 7, -1]
+    assert got["free_blocks"] == [9, 7, -1] and got["status"] == [0, 0, 0, 0]
+    short = ok.plan([16], [17], [[3, -1, -1]], [9], 1, 16, 4)
+    assert short["status"] == [1, 0, 13, 0] and short["lens"] == [16] and short["slots"] == [-1] * 4
+
+
+def test_oracle_append_grows_a_scale():
+    codes, scale = torch.zeros(1, 1, 16, 32, dtype=torch.int8), torch.full((1, 1), 99.0)
+    ok.append(torch.tensor([[[127.0, -63.5, 1.0]]]), [0], codes, scale)      # begins the block: its old scale is gone
+    assert float(scale) == 1.0 and codes[0, 0, 0, :4].tolist() == [127, -64, 1, 0]
+    ok.append(torch.tensor([[[254.0, 3.0, -3.0]]]), [1], codes, scale)
+    assert float(scale) == 2.0 and codes[0, 0, 0, :4].tolist() == [64, -32, 0, 0]
+    assert codes[0, 0, 1, :4].tolist() == [127, 2, -2, 0]                     # 1.5 rounds to the even 2
