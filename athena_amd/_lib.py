@@ -192,7 +192,7 @@ _SIGNATURES = {
     "athena_kv_plan": (c_int, [_P, _P, _P, c_long, c_int, _P, c_int, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _S]),
     "athena_kv8_append": (c_int, [_P, _P, c_long, c_long, c_long, c_long, c_int, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int,
                                   c_int, c_int, _S]),
-    "athena_kv8_attention_workspace_bytes": (c_int64, [c_int] * 9),
+    "athena_kv8_attention_workspace_bytes": (c_int64, [c_int] * 10),
     "athena_kv8_attention": (c_int, [_P, c_long, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_int, _P, c_long, c_int, _P, _P,
                                      c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_long, c_long, _P, _P,
                                      c_int64, _S]),

@@ -10,7 +10,7 @@ FLAGS="--offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wno-unused-result -Wno-inline
 pids=()
 for f in gemm norm attention loss optim misc frontconv layer_tail panel conv2d rnn metrics kv_cache logits; do
   src="$here/$f.hip"; obj="$here/.obj/$f.o"
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$here/common.h" -nt "$obj" ] || [ "$here/gemm_core.h" -nt "$obj" ] || [ "$here/gemm_big.h" -nt "$obj" ] || [ "$here/attention_mfma.h" -nt "$obj" ] || [ "$here/layer_tail_frag.h" -nt "$obj" ] || [ "$here/../../include/athena_hip.h" -nt "$obj" ]; then
+  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$here/common.h" -nt "$obj" ] || [ "$here/gemm_core.h" -nt "$obj" ] || [ "$here/gemm_big.h" -nt "$obj" ] || [ "$here/attention_mfma.h" -nt "$obj" ] || [ "$here/layer_tail_frag.h" -nt "$obj" ] || [ "$here/kv_attention.h" -nt "$obj" ] || [ "$here/../../include/athena_hip.h" -nt "$obj" ]; then
     $HIPCC $FLAGS -c "$src" -o "$obj" &
     pids+=($!)
   fi

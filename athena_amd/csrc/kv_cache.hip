@@ -8,6 +8,7 @@
 // are contracted over the tokens and lie column by column: both are then read from memory straight into
 // matrix-core operands, without a transposition on the way.
 #include "common.h"
+#include "kv_attention.h"
 
 // ---------------------------------------------------------------- block plans
 // One workgroup sums over the requests (new rows, blocks taken, blocks given back), decides whether the
@@ -452,78 +453,43 @@ extern "C" int athena_kv8_append(const void* k, const void* v, long ldk, long ld
 }
 
 // ---------------------------------------------------------------- attention over the cache
-// out[t, head] = sum_j p_j v_j, p = softmax_j(scale * q_t . k_j) over the tokens j of t's sequence that it may
-// see.  One workgroup per (row, head); keys in tiles of 128: a thread scores one key, then the threads take
-// the columns of the output.
-struct KvAttn {
-    const void* q;
-    long ldq, ldq_head;
-    const int8_t *k_codes, *v_codes;
-    const float *k_scale, *v_scale;
-    const int32_t* tables;
-    long ld_tables;
-    const int32_t *lens, *cu_rows;
-    void* out;
-    long ldo, ldo_head;
-    float* lse;             // [N][heads] or null
-    int table_width, num_blocks, B, N, h, hk, dk, block_size, causal;
-    float scale;
+struct KvShape {
+    int rt, row_tiles, splits;
 };
 
-#define KV_TILE 128
-
-template <typename T, int W>
-__global__ __launch_bounds__(KV_TILE) void kv8_attention_kernel(KvAttn a) {
-    __shared__ float sq[W], sp[KV_TILE], red[32];
-    const int b = blockIdx.z, head = blockIdx.y, tid = threadIdx.x;
-    const int lo = min(max(a.cu_rows ? a.cu_rows[b] : b, 0), a.N), hi = min(max(a.cu_rows ? a.cu_rows[b + 1] : b + 1, lo), a.N);
-    const long long most = (long long)a.table_width * a.block_size;
-    const int len = (int)min((long long)max(a.lens[b], 0), most), g = head / (a.h / a.hk);
-    for (int t = lo + blockIdx.x; t < hi; t += gridDim.x) {
-        const T* q = (const T*)a.q + (long)t * a.ldq + (long)head * a.ldq_head;
-        __syncthreads();
-        for (int c = tid; c < W; c += KV_TILE) sq[c] = c < a.dk ? to_f32<T>(q[c]) * a.scale : 0.f;
-        __syncthreads();
-        const int end = a.causal ? min(len, len - (hi - t) + 1) : len;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-        for (int j0 = 0; j0 < end; j0 += KV_TILE) {
-            const int j = j0 + tid;
-            float s = -INFINITY;
-            if (j < end) {
-                const int block = a.tables[(long)b * a.ld_tables + j / a.block_size];
-                if (block >= 0 && block < a.num_blocks) {
-                    const long at = (long)block * a.hk + g;
-                    const int8_t* k = a.k_codes + (at * a.block_size + j % a.block_size) * W;
-                    s = 0.f;
-                    for (int c = 0; c < W; ++c) s = fmaf(sq[c], (float)k[c], s);
-                    s *= a.k_scale[at];
-                }
-            }
-            const float mn = fmaxf(m, block_max(s, red)), base = mn == -INFINITY ? 0.f : mn;
-            const float p = __expf(s - base), alpha = __expf(m - base);
-            sp[tid] = p;
-            l = l * alpha + block_sum(p, red);
-            __syncthreads();
-            o *= alpha;
-            if (tid < W) {
-                for (int i = 0; i < KV_TILE && j0 + i < end; ++i) {
-                    const int block = a.tables[(long)b * a.ld_tables + (j0 + i) / a.block_size];
-                    if (block < 0 || block >= a.num_blocks) continue;
-                    const long at = (long)block * a.hk + g;
-                    o = fmaf(sp[i] * a.v_scale[at], (float)a.v_codes[(at * W + tid) * a.block_size + (j0 + i) % a.block_size], o);
-                }
-            }
-            m = mn;
-        }
-        if (tid < a.dk)
-            ((T*)a.out)[(long)t * a.ldo + (long)head * a.ldo_head + tid] = from_f32<T>(l > 0.f ? o / l : l != l ? l : 0.f);
-        if (a.lse && tid == 0) a.lse[(long)t * a.h + head] = l > 0.f ? m + __logf(l) : l != l ? l : -INFINITY;
-    }
+// Query rows per wave and how far the key axis is split.  A split costs a second launch (the join, about 2 us), so
+// none has fewer than KV_MIN_TILES tiles, and there are as many as fill the chip about three times over.
+static KvShape kv8_shape(int dtype, int B, int max_rows, int h, int hk, int table_width, int block_size, int width) {
+    KvShape s;
+    const long rows = (long)max_rows * (h / hk);
+    const int most = dtype == ATHENA_F32 ? (width == 128 ? 1 : 2) : width == 128 ? 2 : 4;      // what fits the registers
+    s.rt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+    const long tiles = (rows + 16 * s.rt - 1) / (16 * s.rt);
+    s.row_tiles = (int)(tiles < 65536 ? tiles : 65536);
+    const long units = (long)B * hk * s.row_tiles, key_tiles = ((long)table_width * block_size + KV_KEYS - 1) / KV_KEYS;
+    long splits = (1536 + units - 1) / units;
+    const long cap = key_tiles / KV_MIN_TILES;
+    if (splits > cap) splits = cap;
+    s.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    return s;
 }
 
-extern "C" int64_t athena_kv8_attention_workspace_bytes(int B, int max_rows, int N, int h, int hk, int table_width, int block_size,
-                                                        int dk, int width) {
-    return 0;
+extern "C" int64_t athena_kv8_attention_workspace_bytes(int dtype, int B, int max_rows, int N, int h, int hk, int table_width,
+                                                        int block_size, int dk, int width) {
+    if (B <= 0 || max_rows <= 0 || N <= 0 || hk <= 0 || h < hk || table_width <= 0 || block_size <= 0 || dk <= 0) return 0;
+    const KvShape s = kv8_shape(dtype, B, max_rows, h, hk, table_width, block_size, width);
+    return s.splits > 1 ? (int64_t)s.splits * N * h * (dk + 1) * 4 : 0;
+}
+
+template <typename T, int W>
+static void kv8_launch(const KvAttn& a, const KvShape& sh, hipStream_t s) {
+    const long units = ((long)a.B * a.hk + 7) / 8 * 8 * sh.row_tiles * sh.splits;
+    const dim3 grid((unsigned)units), block(256);
+    if (sh.rt == 4) {
+        if constexpr (W < 128 && sizeof(T) == 2) ATHENA_LAUNCH((kv8_attention_kernel<T, W, 4>), grid, block, 0, s, a);
+    } else if (sh.rt == 2) {
+        if constexpr (W < 128 || sizeof(T) == 2) ATHENA_LAUNCH((kv8_attention_kernel<T, W, 2>), grid, block, 0, s, a);
+    } else ATHENA_LAUNCH((kv8_attention_kernel<T, W, 1>), grid, block, 0, s, a);
 }
 
 extern "C" int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, const int8_t* k_codes, const int8_t* v_codes,
@@ -535,7 +501,7 @@ extern "C" int athena_kv8_attention(const void* q, long ldq, long ldq_head, int 
     int rc = kv8_check("athena_kv8_attention", num_blocks, hk, block_size, dk, width);
     if (rc) return rc;
     ATHENA_REQUIRE(B > 0 && B <= 65535 && N >= 0 && max_rows > 0 && h > 0 && h <= 65535 && h % hk == 0 && table_width > 0 &&
-                       (long)table_width * block_size < (1L << 31),
+                       (long)table_width * block_size < (1L << 31) - KV_KEYS * 8,
                    ATHENA_E_SHAPE, "athena_kv8_attention: bad shape B=%d N=%d max_rows=%d heads=%d kv_heads=%d table_width=%d", B, N,
                    max_rows, h, hk, table_width);
     ATHENA_REQUIRE(dtype == ATHENA_F32 || dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_attention: dtype");
@@ -544,19 +510,35 @@ extern "C" int athena_kv8_attention(const void* q, long ldq, long ldq_head, int 
                    "athena_kv8_attention: null operand");
     ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN,
                    "athena_kv8_attention: codes must lie on 16 bytes");
+    if (!cu_rows) max_rows = 1;
+    const KvShape sh = kv8_shape(dtype, B, max_rows, h, hk, table_width, block_size, width);
+    ATHENA_REQUIRE(((long)B * hk + 7) / 8 * 8 * sh.row_tiles * sh.splits < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: too many workgroups");
+    const int64_t need = athena_kv8_attention_workspace_bytes(dtype, B, max_rows, N, h, hk, table_width, block_size, dk, width);
+    ATHENA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), ATHENA_E_SHAPE, "athena_kv8_attention: workspace of %ld bytes, %ld needed",
+                   (long)workspace_bytes, (long)need);
+    const int e = dtype == ATHENA_BF16 ? 2 : 4;
     KvAttn a = {q, ldq, ldq_head, k_codes, v_codes, k_scale, v_scale, tables, ld_tables, lens, cu_rows, out, ldo, ldo_head, lse,
-                table_width, num_blocks, B, N, h, hk, dk, block_size, causal, scale};
-    const dim3 grid(max_rows < 4096 ? max_rows : 4096, h, B), block(KV_TILE);
+                (float*)workspace, (float*)workspace + (sh.splits > 1 ? (long)sh.splits * N * h * dk : 0), table_width, num_blocks, B,
+                N, h, hk, dk, block_size, causal, sh.splits, sh.row_tiles, 0, 0, scale};
+    // whole 16-byte (queries) / four-element (results) accesses where rows, heads and columns allow them
+    a.q_wide = athena_aligned16(q) && ldq * e % 16 == 0 && ldq_head * e % 16 == 0 && dk % 8 == 0;
+    a.out_wide = (uintptr_t)out % (4 * e) == 0 && ldo % 4 == 0 && ldo_head % 4 == 0;
     hipStream_t s = (hipStream_t)stream;
-#define KV_SIMPLE(T)                                                                              \
-    do {                                                                                          \
-        if (width == 32) ATHENA_LAUNCH((kv8_attention_kernel<T, 32>), grid, block, 0, s, a);      \
-        else if (width == 64) ATHENA_LAUNCH((kv8_attention_kernel<T, 64>), grid, block, 0, s, a); \
-        else ATHENA_LAUNCH((kv8_attention_kernel<T, 128>), grid, block, 0, s, a);                 \
+#define KV_LAUNCH(T)                                   \
+    do {                                               \
+        if (width == 32) kv8_launch<T, 32>(a, sh, s);  \
+        else if (width == 64) kv8_launch<T, 64>(a, sh, s); \
+        else kv8_launch<T, 128>(a, sh, s);             \
     } while (0)
-    if (dtype == ATHENA_BF16) KV_SIMPLE(bf16_t);
-    else KV_SIMPLE(float);
-#undef KV_SIMPLE
+    if (dtype == ATHENA_BF16) KV_LAUNCH(bf16_t);
+    else KV_LAUNCH(float);
+#undef KV_LAUNCH
     ATHENA_CHECK_LAUNCH("athena_kv8_attention");
+    if (sh.splits > 1) {
+        const dim3 grid(max_rows < 4096 ? max_rows : 4096, (h + 3) / 4, B);
+        if (dtype == ATHENA_BF16) ATHENA_LAUNCH(kv8_join_kernel<bf16_t>, grid, dim3(256), 0, s, a);
+        else ATHENA_LAUNCH(kv8_join_kernel<float>, grid, dim3(256), 0, s, a);
+        ATHENA_CHECK_LAUNCH("athena_kv8_attention (join)");
+    }
     return ATHENA_OK;
 }

@@ -1391,7 +1391,7 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows=N
         raise RuntimeError("athena_amd.kv8_attention: lse must be contiguous fp32 [%d, %d]" % (n, h))
     _here("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows, out, lse)
     lib = _lib.load()
-    need = lib.athena_kv8_attention_workspace_bytes(B, max_rows, n, h, hk, width, bs, dk, w)
+    need = lib.athena_kv8_attention_workspace_bytes(dt(q), B, max_rows, n, h, hk, width, bs, dk, w)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _lib.check(lib.athena_kv8_attention(_ptr(q), ldq, ldq_h, dt(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale),
                                         nb, bs, w, _ptr(tables), ldt, width, _ptr(lens), _ptr(cu_rows), B, max_rows, n, h, hk,

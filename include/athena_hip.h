@@ -798,8 +798,8 @@ int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, lon
  * lse: fp32 [N][h], natural logarithm of the sum of exponentials, or null.
  * ld_tables may be 0: every sequence then reads the same blocks.
  * ``workspace``: athena_kv8_attention_workspace_bytes (0: none is needed). */
-int64_t athena_kv8_attention_workspace_bytes(int B, int max_rows, int N, int h, int hk, int table_width, int block_size,
-                                             int dk, int width);
+int64_t athena_kv8_attention_workspace_bytes(int dtype, int B, int max_rows, int N, int h, int hk, int table_width,
+                                             int block_size, int dk, int width);
 int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, const int8_t* k_codes, const int8_t* v_codes,
                          const float* k_scale, const float* v_scale, int num_blocks, int block_size, int width,
                          const int32_t* tables, long ld_tables, int table_width, const int32_t* lens,
