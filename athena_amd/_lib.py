@@ -5,6 +5,7 @@ or unloadable library raises at first use with the command that builds it.
 """
 import ctypes
 import os
+import struct
 from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_long,
                     c_size_t, c_uint32, c_uint64, c_void_p)
 
@@ -90,6 +91,14 @@ class AdamCfg(Structure):
         ("schedule", c_float), ("initial_lr", c_float), ("start_decay_steps", c_float), ("final_lr", c_float),
     ]
 
+
+# The descriptors of the decoding entry points, packed in one go: a decoding step issues many small calls, and setting
+# some thirty Structure fields one by one takes longer than such a kernel runs.  Pointers (0 = null), then
+# 64-bit, then 32-bit members, as include/athena_hip.h declares them.
+KvPlanDesc = struct.Struct("@12Qq6i")              # athena_kv_plan_desc
+Kv8AppendDesc = struct.Struct("@7Q4q8i")           # athena_kv8_append_desc
+Kv8AttentionDesc = struct.Struct("@11Q6q12i2f")    # athena_kv8_attention_desc
+LogitsDesc = struct.Struct("@11Q7q6i")             # athena_logits_desc
 
 _P = c_void_p
 _S = c_void_p   # stream
@@ -189,15 +198,11 @@ _SIGNATURES = {
     "athena_cast": (c_int, [_P, c_int, _P, c_int, c_long, _S]),
     "athena_copy_many": (c_int, [_P, _P, _P, c_int, _S]),
     "athena_axpby": (c_int, [c_float, _P, c_float, _P, c_long, c_int, _S]),
-    "athena_kv_plan": (c_int, [_P, _P, _P, c_long, c_int, _P, c_int, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _S]),
-    "athena_kv8_append": (c_int, [_P, _P, c_long, c_long, c_long, c_long, c_int, _P, c_int, _P, _P, _P, _P, c_int, c_int, c_int,
-                                  c_int, c_int, _S]),
-    "athena_kv8_attention_workspace_bytes": (c_int64, [c_int] * 10),
-    "athena_kv8_attention": (c_int, [_P, c_long, c_long, c_int, _P, _P, _P, _P, c_int, c_int, c_int, _P, c_long, c_int, _P, _P,
-                                     c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_long, c_long, _P, _P,
-                                     c_int64, _S]),
-    "athena_logits_process": (c_int, [_P, c_long, c_int, c_int, c_int, _P, c_long, c_int, _P, _P, _P, _P, _P, c_long, _P,
-                                      c_long, _P, c_long, c_int, _P, c_long, _P, c_long, _S]),
+    "athena_kv_plan": (c_int, [c_char_p, _S]),
+    "athena_kv8_append": (c_int, [c_char_p, _S]),
+    "athena_kv8_attention_workspace_bytes": (c_int64, [c_char_p]),
+    "athena_kv8_attention": (c_int, [c_char_p, _S]),
+    "athena_logits_process": (c_int, [c_char_p, _S]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

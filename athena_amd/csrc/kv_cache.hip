@@ -179,25 +179,31 @@ __global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a) {
     plan_fill(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
-extern "C" int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int32_t* tables, long ld_tables, int table_width,
-                              int32_t* free_blocks, int free_capacity, const int32_t* free_count, int B, int block_size,
-                              int rows, int32_t* cu_rows, int32_t* slots, int32_t* positions, int32_t* lens_out,
-                              int32_t* free_count_out, int32_t* status, int32_t* work, athena_stream_t stream) {
-    ATHENA_REQUIRE(B > 0 && table_width > 0 && free_capacity > 0 && rows >= 0 && ld_tables >= table_width, ATHENA_E_SHAPE,
-                   "athena_kv_plan: bad shape B=%d table_width=%d free_capacity=%d rows=%d ld=%ld", B, table_width,
-                   free_capacity, rows, ld_tables);
-    ATHENA_REQUIRE(block_size == 16 || block_size == 32 || block_size == 64 || block_size == 128, ATHENA_E_UNSUPPORTED,
-                   "athena_kv_plan: block size %d not in {16, 32, 64, 128}", block_size);
-    ATHENA_REQUIRE((long)table_width * block_size < (1L << 31), ATHENA_E_SHAPE, "athena_kv_plan: table too wide");
-    ATHENA_REQUIRE(lens && new_rows && tables && free_blocks && free_count && cu_rows && (slots || !rows) && (positions || !rows) &&
-                       lens_out && free_count_out && status && work,
+extern "C" int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stream) {
+    ATHENA_REQUIRE(d, ATHENA_E_SHAPE, "athena_kv_plan: null descriptor");
+    ATHENA_REQUIRE(d->B > 0 && d->table_width > 0 && d->free_capacity > 0 && d->rows >= 0 && d->ld_tables >= d->table_width,
+                   ATHENA_E_SHAPE, "athena_kv_plan: bad shape B=%d table_width=%d free_capacity=%d rows=%d ld=%ld", d->B,
+                   d->table_width, d->free_capacity, d->rows, (long)d->ld_tables);
+    const int bs = d->block_size;
+    ATHENA_REQUIRE(bs == 16 || bs == 32 || bs == 64 || bs == 128, ATHENA_E_UNSUPPORTED,
+                   "athena_kv_plan: block size %d not in {16, 32, 64, 128}", bs);
+    ATHENA_REQUIRE((long)d->table_width * bs < (1L << 31), ATHENA_E_SHAPE, "athena_kv_plan: table too wide");
+    ATHENA_REQUIRE(d->lens && d->new_rows && d->tables && d->free_blocks && d->free_count && d->cu_rows &&
+                       ((d->slots && d->positions) || !d->rows) && d->lens_out && d->free_count_out && d->status && d->work,
                    ATHENA_E_SHAPE, "athena_kv_plan: null operand");
-    PlanArgs a = {lens, new_rows, tables, ld_tables, free_blocks, free_count, cu_rows, slots, positions, lens_out,
-                  free_count_out, status, work, work + 2L * B + 3, B, table_width, free_capacity, block_size, rows};
+    PlanArgs a = {d->lens, d->new_rows, d->tables, d->ld_tables, d->free_blocks, d->free_count, d->cu_rows, d->slots, d->positions,
+                  d->lens_out, d->free_count_out, d->status, d->work, d->work + 2L * d->B + 3, d->B, d->table_width,
+                  d->free_capacity, bs, d->rows};
     hipStream_t s = (hipStream_t)stream;
-    const int fill = 1;
+    // one workgroup fills up to four rows a thread and 16 requests a wave itself; beyond that a launch of many is faster
+    const int fill = d->rows <= 4 * PLAN_THREADS && d->B <= 16 * (PLAN_THREADS / 64);
     ATHENA_LAUNCH(kv_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, s, a, fill);
     ATHENA_CHECK_LAUNCH("athena_kv_plan");
+    if (!fill) {
+        const long units = (long)d->B * 64 > d->rows ? (long)d->B * 64 : d->rows, wgs = (units + 255) / 256;
+        ATHENA_LAUNCH(kv_plan_fill_kernel, dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, s, a);
+        ATHENA_CHECK_LAUNCH("athena_kv_plan (fill)");
+    }
     return ATHENA_OK;
 }
 
@@ -416,20 +422,25 @@ static int kv8_check(const char* name, int num_blocks, int hk, int block_size, i
     return ATHENA_OK;
 }
 
-extern "C" int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, long ldv, long ldv_head, int dtype,
-                                 const int32_t* slots, int N, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
-                                 int num_blocks, int hk, int block_size, int dk, int width, athena_stream_t stream) {
+extern "C" int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_t stream) {
+    ATHENA_REQUIRE(d, ATHENA_E_SHAPE, "athena_kv8_append: null descriptor");
+    const int num_blocks = d->num_blocks, hk = d->hk, block_size = d->block_size, dk = d->dk, width = d->width, N = d->N;
     int rc = kv8_check("athena_kv8_append", num_blocks, hk, block_size, dk, width);
     if (rc) return rc;
     ATHENA_REQUIRE(N >= 0, ATHENA_E_SHAPE, "athena_kv8_append: N=%d", N);
+    ATHENA_REQUIRE(d->dtype == ATHENA_F32 || d->dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_append: dtype");
     if (N == 0) return ATHENA_OK;
+    const void *k = d->k, *v = d->v;
+    const long ldk = d->ldk, ldk_head = d->ldk_head, ldv = d->ldv, ldv_head = d->ldv_head;
+    const int32_t* slots = d->slots;
+    int8_t *k_codes = d->k_codes, *v_codes = d->v_codes;
+    float *k_scale = d->k_scale, *v_scale = d->v_scale;
     ATHENA_REQUIRE(k && v && slots && k_codes && v_codes && k_scale && v_scale, ATHENA_E_SHAPE, "athena_kv8_append: null operand");
     ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN, "athena_kv8_append: codes must lie on 16 bytes");
-    ATHENA_REQUIRE(dtype == ATHENA_F32 || dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_append: dtype");
     const int per = (long)N * hk <= 4096 ? 1 : 16;
     const dim3 grid((N + per - 1) / per, hk), block(per == 1 ? 128 : 256);
     const long end = (long)num_blocks * block_size;
-    const size_t two = dtype == ATHENA_BF16 ? 4 : 8;        // two elements in one load where rows and heads begin on them
+    const size_t two = d->dtype == ATHENA_BF16 ? 4 : 8;        // two elements in one load where rows and heads begin on them
     const int kp = (uintptr_t)k % two == 0 && ldk % 2 == 0 && ldk_head % 2 == 0;
     const int vp = (uintptr_t)v % two == 0 && ldv % 2 == 0 && ldv_head % 2 == 0;
 #define KV_APPEND(T, W)                                                                                                     \
@@ -444,7 +455,7 @@ extern "C" int athena_kv8_append(const void* k, const void* v, long ldk, long ld
         else if (width == 64) KV_APPEND(T, 64); \
         else KV_APPEND(T, 128);            \
     } while (0)
-    if (dtype == ATHENA_BF16) KV_APPEND_W(bf16_t);
+    if (d->dtype == ATHENA_BF16) KV_APPEND_W(bf16_t);
     else KV_APPEND_W(float);
 #undef KV_APPEND_W
 #undef KV_APPEND
@@ -459,14 +470,14 @@ struct KvShape {
 
 // Query rows per wave and how far the key axis is split.  A split costs a second launch (the join, about 2 us), so
 // none has fewer than KV_MIN_TILES tiles, and there are as many as fill the chip about three times over.
-static KvShape kv8_shape(int dtype, int B, int max_rows, int h, int hk, int table_width, int block_size, int width) {
+static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     KvShape s;
-    const long rows = (long)max_rows * (h / hk);
-    const int most = dtype == ATHENA_F32 ? (width == 128 ? 1 : 2) : width == 128 ? 2 : 4;      // what fits the registers
+    const long rows = (long)(d->cu_rows ? d->max_rows : 1) * (d->h / d->hk);
+    const int most = d->dtype == ATHENA_F32 ? (d->width == 128 ? 1 : 2) : d->width == 128 ? 2 : 4;     // what fits the registers
     s.rt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
     const long tiles = (rows + 16 * s.rt - 1) / (16 * s.rt);
     s.row_tiles = (int)(tiles < 65536 ? tiles : 65536);
-    const long units = (long)B * hk * s.row_tiles, key_tiles = ((long)table_width * block_size + KV_KEYS - 1) / KV_KEYS;
+    const long units = (long)d->B * d->hk * s.row_tiles, key_tiles = ((long)d->table_width * d->block_size + KV_KEYS - 1) / KV_KEYS;
     long splits = (1536 + units - 1) / units;
     const long cap = key_tiles / KV_MIN_TILES;
     if (splits > cap) splits = cap;
@@ -474,11 +485,12 @@ static KvShape kv8_shape(int dtype, int B, int max_rows, int h, int hk, int tabl
     return s;
 }
 
-extern "C" int64_t athena_kv8_attention_workspace_bytes(int dtype, int B, int max_rows, int N, int h, int hk, int table_width,
-                                                        int block_size, int dk, int width) {
-    if (B <= 0 || max_rows <= 0 || N <= 0 || hk <= 0 || h < hk || table_width <= 0 || block_size <= 0 || dk <= 0) return 0;
-    const KvShape s = kv8_shape(dtype, B, max_rows, h, hk, table_width, block_size, width);
-    return s.splits > 1 ? (int64_t)s.splits * N * h * (dk + 1) * 4 : 0;
+extern "C" int64_t athena_kv8_attention_workspace_bytes(const athena_kv8_attention_desc* d) {
+    if (!d || d->B <= 0 || d->max_rows <= 0 || d->N <= 0 || d->hk <= 0 || d->h < d->hk || d->table_width <= 0 || d->block_size <= 0 ||
+        d->dk <= 0)
+        return 0;
+    const KvShape s = kv8_shape(d);
+    return s.splits > 1 ? (int64_t)s.splits * d->N * d->h * (d->dk + 1) * 4 : 0;
 }
 
 template <typename T, int W>
@@ -492,51 +504,49 @@ static void kv8_launch(const KvAttn& a, const KvShape& sh, hipStream_t s) {
     } else ATHENA_LAUNCH((kv8_attention_kernel<T, W, 1>), grid, block, 0, s, a);
 }
 
-extern "C" int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, const int8_t* k_codes, const int8_t* v_codes,
-                                    const float* k_scale, const float* v_scale, int num_blocks, int block_size, int width,
-                                    const int32_t* tables, long ld_tables, int table_width, const int32_t* lens,
-                                    const int32_t* cu_rows, int B, int max_rows, int N, int h, int hk, int dk, int causal,
-                                    float scale, void* out, long ldo, long ldo_head, float* lse, void* workspace,
-                                    int64_t workspace_bytes, athena_stream_t stream) {
-    int rc = kv8_check("athena_kv8_attention", num_blocks, hk, block_size, dk, width);
+extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_stream_t stream) {
+    ATHENA_REQUIRE(d, ATHENA_E_SHAPE, "athena_kv8_attention: null descriptor");
+    int rc = kv8_check("athena_kv8_attention", d->num_blocks, d->hk, d->block_size, d->dk, d->width);
     if (rc) return rc;
-    ATHENA_REQUIRE(B > 0 && B <= 65535 && N >= 0 && max_rows > 0 && h > 0 && h <= 65535 && h % hk == 0 && table_width > 0 &&
-                       (long)table_width * block_size < (1L << 31) - KV_KEYS * 8,
+    const int B = d->B, N = d->N, h = d->h, hk = d->hk, e = d->dtype == ATHENA_BF16 ? 2 : 4;
+    ATHENA_REQUIRE(B > 0 && B <= 65535 && N >= 0 && d->max_rows > 0 && h > 0 && h <= 65535 && h % hk == 0 && d->table_width > 0 &&
+                       (long)d->table_width * d->block_size < (1L << 31) - KV_KEYS * 8,
                    ATHENA_E_SHAPE, "athena_kv8_attention: bad shape B=%d N=%d max_rows=%d heads=%d kv_heads=%d table_width=%d", B, N,
-                   max_rows, h, hk, table_width);
-    ATHENA_REQUIRE(dtype == ATHENA_F32 || dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_attention: dtype");
+                   d->max_rows, h, hk, d->table_width);
+    ATHENA_REQUIRE(d->dtype == ATHENA_F32 || d->dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_attention: dtype");
     if (N == 0) return ATHENA_OK;
-    ATHENA_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && tables && lens && out, ATHENA_E_SHAPE,
+    ATHENA_REQUIRE(d->q && d->k_codes && d->v_codes && d->k_scale && d->v_scale && d->tables && d->lens && d->out, ATHENA_E_SHAPE,
                    "athena_kv8_attention: null operand");
-    ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN,
+    ATHENA_REQUIRE(d->cu_rows || N == B, ATHENA_E_SHAPE, "athena_kv8_attention: %d rows for %d sequences need cu_rows", N, B);
+    ATHENA_REQUIRE(athena_aligned16(d->k_codes) && athena_aligned16(d->v_codes), ATHENA_E_ALIGN,
                    "athena_kv8_attention: codes must lie on 16 bytes");
-    if (!cu_rows) max_rows = 1;
-    const KvShape sh = kv8_shape(dtype, B, max_rows, h, hk, table_width, block_size, width);
+    const KvShape sh = kv8_shape(d);
     ATHENA_REQUIRE(((long)B * hk + 7) / 8 * 8 * sh.row_tiles * sh.splits < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: too many workgroups");
-    const int64_t need = athena_kv8_attention_workspace_bytes(dtype, B, max_rows, N, h, hk, table_width, block_size, dk, width);
-    ATHENA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), ATHENA_E_SHAPE, "athena_kv8_attention: workspace of %ld bytes, %ld needed",
-                   (long)workspace_bytes, (long)need);
-    const int e = dtype == ATHENA_BF16 ? 2 : 4;
-    KvAttn a = {q, ldq, ldq_head, k_codes, v_codes, k_scale, v_scale, tables, ld_tables, lens, cu_rows, out, ldo, ldo_head, lse,
-                (float*)workspace, (float*)workspace + (sh.splits > 1 ? (long)sh.splits * N * h * dk : 0), table_width, num_blocks, B,
-                N, h, hk, dk, block_size, causal, sh.splits, sh.row_tiles, 0, 0, scale};
+    const int64_t need = athena_kv8_attention_workspace_bytes(d);
+    ATHENA_REQUIRE(need == 0 || (d->workspace && d->workspace_bytes >= need), ATHENA_E_SHAPE,
+                   "athena_kv8_attention: workspace of %ld bytes, %ld needed", (long)d->workspace_bytes, (long)need);
+    float* part = (float*)d->workspace;
     // whole 16-byte (queries) / four-element (results) accesses where rows, heads and columns allow them
-    a.q_wide = athena_aligned16(q) && ldq * e % 16 == 0 && ldq_head * e % 16 == 0 && dk % 8 == 0;
-    a.out_wide = (uintptr_t)out % (4 * e) == 0 && ldo % 4 == 0 && ldo_head % 4 == 0;
+    const int q_wide = athena_aligned16(d->q) && d->ldq * e % 16 == 0 && d->ldq_head * e % 16 == 0 && d->dk % 8 == 0;
+    const int out_wide = (uintptr_t)d->out % (4 * e) == 0 && d->ldo % 4 == 0 && d->ldo_head % 4 == 0;
+    KvAttn a = {d->q, d->ldq, d->ldq_head, d->k_codes, d->v_codes, d->k_scale, d->v_scale, d->tables, d->ld_tables, d->lens, d->cu_rows,
+                d->out, d->ldo, d->ldo_head, d->lse, part, part + (sh.splits > 1 ? (long)sh.splits * N * h * d->dk : 0), d->table_width,
+                d->num_blocks, B, N, h, hk, d->dk, d->block_size, d->causal, sh.splits, sh.row_tiles, q_wide, out_wide, d->scale};
     hipStream_t s = (hipStream_t)stream;
-#define KV_LAUNCH(T)                                   \
-    do {                                               \
-        if (width == 32) kv8_launch<T, 32>(a, sh, s);  \
-        else if (width == 64) kv8_launch<T, 64>(a, sh, s); \
-        else kv8_launch<T, 128>(a, sh, s);             \
+#define KV_LAUNCH(T)                                      \
+    do {                                                  \
+        if (d->width == 32) kv8_launch<T, 32>(a, sh, s);  \
+        else if (d->width == 64) kv8_launch<T, 64>(a, sh, s); \
+        else kv8_launch<T, 128>(a, sh, s);                \
     } while (0)
-    if (dtype == ATHENA_BF16) KV_LAUNCH(bf16_t);
+    if (d->dtype == ATHENA_BF16) KV_LAUNCH(bf16_t);
     else KV_LAUNCH(float);
 #undef KV_LAUNCH
     ATHENA_CHECK_LAUNCH("athena_kv8_attention");
     if (sh.splits > 1) {
-        const dim3 grid(max_rows < 4096 ? max_rows : 4096, (h + 3) / 4, B);
-        if (dtype == ATHENA_BF16) ATHENA_LAUNCH(kv8_join_kernel<bf16_t>, grid, dim3(256), 0, s, a);
+        const int rows = d->cu_rows ? d->max_rows : 1;
+        const dim3 grid(rows < 4096 ? rows : 4096, (h + 3) / 4, B);
+        if (d->dtype == ATHENA_BF16) ATHENA_LAUNCH(kv8_join_kernel<bf16_t>, grid, dim3(256), 0, s, a);
         else ATHENA_LAUNCH(kv8_join_kernel<float>, grid, dim3(256), 0, s, a);
         ATHENA_CHECK_LAUNCH("athena_kv8_attention (join)");
     }

@@ -4,50 +4,52 @@
 // For class v of row r with c = how often v occurs in the row's history:
 //   x = logit;  c > 0: x = x > 0 ? x / repetition : x * repetition;  x -= frequency c + presence [c > 0];
 //   x += bias;  -inf where the row's mask does not allow v.
-// A workgroup takes one tile of classes of one row: occurrences of the tile's classes are counted in LDS from
-// the history (whole-number atomics: their order does not matter), classes with a bias of their own carry a
-// flag in the counter's top bit, and the tile's logits then pass once.  Bound by the logits' way in and out;
-// the history is read again by every tile of a row, from the L2.
+// A workgroup takes one tile of classes of one row.  Its logits are requested first; while they travel, occurrences of
+// the tile's classes are counted in LDS from the history (whole-number atomics: their order does not matter) and classes with
+// a bias of their own get a flag in the counter's top bit.  Then the tile passes once, 16 bytes a lane.  Bound by the
+// logits' way in and out; the history is read again by every tile of a row, from the L2, so tiles are large (8192) where
+// there are enough of them to fill the chip and 1024 (fp32) / 2048 (bf16) where there are not.
 struct LogitsArgs {
     const void* logits;
     void* out;
     const int32_t *history, *history_len, *bias_ids, *allowed;
     const float *repetition, *presence, *frequency, *bias, *bias_values;
     long ldl, ldo, ld_history, ld_bias, ld_bias_ids, ld_bias_values, ld_allowed;
-    int R, V, L, nb, tile;
+    int R, V, L, nb, wide;
 };
 
-#define LOGITS_TILE 8192
 #define LOGITS_BIASED 0x80000000u
 
-template <typename T>
-__device__ __forceinline__ float logits_one(const LogitsArgs& a, int r, int v, float x, unsigned c, float rep, float pres, float freq,
-                                            unsigned mask_word) {
-    const unsigned n = c & ~LOGITS_BIASED;
-    if (n) {
-        x = x > 0.f ? x / rep : x * rep;
-        x = x - freq * (float)n - pres;
-    }
-    if (a.bias) x += a.bias[(long)r * a.ld_bias + v];
-    if (c & LOGITS_BIASED) {
-        float own = 0.f;                        // entries of one class add up in their order
-        for (int j = 0; j < a.nb; ++j)
-            if (a.bias_ids[(long)r * a.ld_bias_ids + j] == v) own += a.bias_values[(long)r * a.ld_bias_values + j];
-        x += own;
-    }
-    return (mask_word >> (v & 31)) & 1u ? x : -INFINITY;
-}
-
-template <typename T>
+// NB vectors of 16 bytes per thread
+template <typename T, int NB>
 __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
-    extern __shared__ unsigned count[];
-    const int r = blockIdx.y, v0 = blockIdx.x * a.tile, nv = min(a.tile, a.V - v0), tid = threadIdx.x;
-    for (int i = tid; i < nv; i += 256) count[i] = 0;
+    constexpr int E = 16 / sizeof(T), TILE = 256 * E * NB;
+    __shared__ __attribute__((aligned(16))) unsigned count[TILE];
+    struct alignas(16) Vec { T e[E]; };
+    const int r = blockIdx.y, v0 = blockIdx.x * TILE, nv = min(TILE, a.V - v0), tid = threadIdx.x;
+    const T* in = (const T*)a.logits + (long)r * a.ldl + v0;
+    T* out = (T*)a.out + (long)r * a.ldo + v0;
+    Vec x[NB];
+    unsigned mask[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int i = (b * 256 + tid) * E;
+        mask[b] = a.allowed && i < nv ? (unsigned)a.allowed[(long)r * a.ld_allowed + ((v0 + i) >> 5)] : ~0u;
+        if (a.wide && i + E <= nv) x[b] = *(const Vec*)(in + i);
+        else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[b].e[e] = i + e < nv ? in[i + e] : from_f32<T>(0.f);
+        }
+    }
+#pragma unroll
+    for (int i = tid * 4; i < TILE; i += 1024) *(uint4*)&count[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     if (a.history) {
         const int n = a.history_len ? min(max(a.history_len[r], 0), a.L) : a.L;
+        const int32_t* ids = a.history + (long)r * a.ld_history;
+#pragma unroll 4
         for (int i = tid; i < n; i += 256) {
-            const unsigned at = (unsigned)a.history[(long)r * a.ld_history + i] - (unsigned)v0;
+            const unsigned at = (unsigned)ids[i] - (unsigned)v0;
             if (at < (unsigned)nv) atomicAdd(&count[at], 1u);
         }
     }
@@ -58,31 +60,63 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
     __syncthreads();
     const float rep = a.repetition ? a.repetition[r] : 1.f, pres = a.presence ? a.presence[r] : 0.f,
                 freq = a.frequency ? a.frequency[r] : 0.f;
-    const T* in = (const T*)a.logits + (long)r * a.ldl + v0;
-    T* out = (T*)a.out + (long)r * a.ldo + v0;
-    const int32_t* allowed = a.allowed ? a.allowed + (long)r * a.ld_allowed : nullptr;
-    for (int i = tid; i < nv; i += 256) {
-        const unsigned m = allowed ? (unsigned)allowed[(v0 + i) >> 5] : ~0u;
-        out[i] = from_f32<T>(logits_one<T>(a, r, v0 + i, to_f32<T>(in[i]), count[i], rep, pres, freq, m));
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int i = (b * 256 + tid) * E;
+        if (i >= nv) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int v = v0 + i + e;
+            const unsigned c = count[i + e], n = c & ~LOGITS_BIASED;
+            float y = to_f32<T>(x[b].e[e]);
+            if (n) {
+                y = y > 0.f ? y / rep : y * rep;
+                y = y - freq * (float)n - pres;
+            }
+            if (a.bias && i + e < nv) y += a.bias[(long)r * a.ld_bias + v];
+            if (c & LOGITS_BIASED) {
+                float own = 0.f;                // entries of one class add up in their order
+                for (int j = 0; j < a.nb; ++j)
+                    if (a.bias_ids[(long)r * a.ld_bias_ids + j] == v) own += a.bias_values[(long)r * a.ld_bias_values + j];
+                y += own;
+            }
+            x[b].e[e] = from_f32<T>((mask[b] >> (v & 31)) & 1u ? y : -INFINITY);
+        }
+        if (a.wide && i + E <= nv) *(Vec*)(out + i) = x[b];
+        else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (i + e < nv) out[i + e] = x[b].e[e];
+        }
     }
 }
 
-extern "C" int athena_logits_process(const void* logits, long ldl, int dtype, int R, int V, const int32_t* history, long ld_history,
-                                     int L, const int32_t* history_len, const float* repetition, const float* presence,
-                                     const float* frequency, const float* bias, long ld_bias, const int32_t* bias_ids,
-                                     long ld_bias_ids, const float* bias_values, long ld_bias_values, int nb,
-                                     const int32_t* allowed, long ld_allowed, void* out, long ldo, athena_stream_t stream) {
-    ATHENA_REQUIRE(R >= 0 && R <= 65535 && V > 0 && L >= 0 && nb >= 0, ATHENA_E_SHAPE,
-                   "athena_logits_process: bad shape R=%d V=%d L=%d biases=%d", R, V, L, nb);
-    ATHENA_REQUIRE(dtype == ATHENA_F32 || dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_logits_process: dtype");
+extern "C" int athena_logits_process(const athena_logits_desc* d, athena_stream_t stream) {
+    ATHENA_REQUIRE(d, ATHENA_E_SHAPE, "athena_logits_process: null descriptor");
+    const int R = d->R, V = d->V;
+    ATHENA_REQUIRE(R >= 0 && R <= 65535 && V > 0 && d->L >= 0 && d->nb >= 0, ATHENA_E_SHAPE,
+                   "athena_logits_process: bad shape R=%d V=%d L=%d biases=%d", R, V, d->L, d->nb);
+    ATHENA_REQUIRE(d->dtype == ATHENA_F32 || d->dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_logits_process: dtype");
     if (R == 0) return ATHENA_OK;
-    ATHENA_REQUIRE(logits && out && (nb == 0 || (bias_ids && bias_values)), ATHENA_E_SHAPE, "athena_logits_process: null operand");
-    ATHENA_REQUIRE(ldl >= V && ldo >= V, ATHENA_E_SHAPE, "athena_logits_process: leading dimension too small");
-    LogitsArgs a = {logits, out, history, history_len, bias_ids, allowed, repetition, presence, frequency, bias, bias_values,
-                    ldl, ldo, ld_history, ld_bias, ld_bias_ids, ld_bias_values, ld_allowed, R, V, history ? L : 0, nb, LOGITS_TILE};
-    const dim3 grid((V + a.tile - 1) / a.tile, R);
-    if (dtype == ATHENA_BF16) ATHENA_LAUNCH(logits_process_kernel<bf16_t>, grid, dim3(256), a.tile * 4, (hipStream_t)stream, a);
-    else ATHENA_LAUNCH(logits_process_kernel<float>, grid, dim3(256), a.tile * 4, (hipStream_t)stream, a);
+    ATHENA_REQUIRE(d->logits && d->out && (d->nb == 0 || (d->bias_ids && d->bias_values)), ATHENA_E_SHAPE,
+                   "athena_logits_process: null operand");
+    ATHENA_REQUIRE(d->ldl >= V && d->ldo >= V, ATHENA_E_SHAPE, "athena_logits_process: leading dimension too small");
+    LogitsArgs a = {d->logits, d->out, d->history, d->history_len, d->bias_ids, d->allowed, d->repetition, d->presence, d->frequency,
+                    d->bias, d->bias_values, d->ldl, d->ldo, d->ld_history, d->ld_bias, d->ld_bias_ids, d->ld_bias_values,
+                    d->ld_allowed, R, V, d->history ? d->L : 0, d->nb, 0};
+    const int e = d->dtype == ATHENA_BF16 ? 2 : 4;
+    a.wide = athena_aligned16(d->logits) && athena_aligned16(d->out) && (R == 1 || (d->ldl * e % 16 == 0 && d->ldo * e % 16 == 0));
+    const bool large = (long)R * ((V + 8191) / 8192) >= 512;
+    const int tile = large ? 8192 : 4096 / e;
+    const dim3 grid((V + tile - 1) / tile, R);
+    hipStream_t s = (hipStream_t)stream;
+    if (d->dtype == ATHENA_BF16) {
+        if (large) ATHENA_LAUNCH((logits_process_kernel<bf16_t, 4>), grid, dim3(256), 0, s, a);
+        else ATHENA_LAUNCH((logits_process_kernel<bf16_t, 1>), grid, dim3(256), 0, s, a);
+    } else {
+        if (large) ATHENA_LAUNCH((logits_process_kernel<float, 8>), grid, dim3(256), 0, s, a);
+        else ATHENA_LAUNCH((logits_process_kernel<float, 1>), grid, dim3(256), 0, s, a);
+    }
     ATHENA_CHECK_LAUNCH("athena_logits_process");
     return ATHENA_OK;
 }

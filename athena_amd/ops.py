@@ -1265,31 +1265,45 @@ def axpby(a, x, b, y):
 
 
 # ------------------------------------------------------------------------------------------ decoding: cache, logits
+# A decoding step issues these calls many times on little work, so the checks look at every property once and the
+# arguments travel in one packed descriptor (see _lib).
 KV8_WIDTHS = (32, 64, 128)
 KV8_BLOCKS = (16, 32, 64, 128)
+_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+_I32, _I8, _FP32 = torch.int32, torch.int8, torch.float32
+
+
+def _refuse(name, what, *args):
+    raise RuntimeError("athena_amd.%s: %s" % (name, what % args if args else what))
 
 
 def _here(name, *tensors):
-    """Every given tensor lives on the current GPU (kernels go to its current stream)."""
+    """The raw current stream, when every given tensor lives on the current GPU (kernels go to its stream)."""
     here = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != here:
-            raise RuntimeError("athena_amd.%s: tensors must live on the current GPU, cuda:%d (got %s)" % (name, here, t.device))
+            _refuse(name, "tensors must live on the current GPU, cuda:%d (got %s)", here, t.device)
+    return torch._C._cuda_getCurrentRawStream(here)
 
 
-def _ints(name, **tensors):
-    """Contiguous int32 tensors of (at least) the given number of elements: name=(tensor, elements)."""
-    for what, (t, n) in tensors.items():
-        if t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous():
-            raise RuntimeError("athena_amd.%s: %s must be contiguous int32 of %d elements" % (name, what, n))
+def _code(name, t):
+    c = _CODES.get(t.dtype)
+    if c is None:
+        raise TypeError("athena_amd.%s: unsupported dtype %s" % (name, t.dtype))
+    return c
+
+
+def _int_vector(name, what, t, n):
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous():
+        _refuse(name, "%s must be contiguous int32 of %d elements", what, n)
 
 
 def _tables(name, tables, B):
     """(leading dimension, width) of a table of blocks."""
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != B or tables.shape[1] < 1 or \
-            (tables.shape[1] > 1 and tables.stride(1) != 1):
-        raise RuntimeError("athena_amd.%s: tables must be int32 [%d, blocks] with rows in one piece" % (name, B))
-    return tables.stride(0), tables.shape[1]
+    shape, stride = tables.shape, tables.stride()
+    if tables.dtype is not _I32 or len(shape) != 2 or shape[0] != B or shape[1] < 1 or (stride[1] != 1 and shape[1] > 1):
+        _refuse(name, "tables must be int32 [%d, blocks] with rows in one piece", B)
+    return stride[0], shape[1]
 
 
 def kv8_width(head_size):
@@ -1311,56 +1325,65 @@ def kv_plan(lens, new_rows, tables, free_blocks, free_count, block_size, rows, i
     fit and nothing was changed."""
     B = lens.numel()
     ldt, width = _tables("kv_plan", tables, B)
-    _ints("kv_plan", lens=(lens, 1), new_rows=(new_rows, B), free_blocks=(free_blocks, 1), free_count=(free_count, 1))
-    _here("kv_plan", lens, new_rows, tables, free_blocks, free_count)
+    if width > 1 and ldt < width and B > 1:
+        _refuse("kv_plan", "tables must not share rows")
+    _int_vector("kv_plan", "lens", lens, 1)
+    _int_vector("kv_plan", "new_rows", new_rows, B)
+    _int_vector("kv_plan", "free_blocks", free_blocks, 1)
+    _int_vector("kv_plan", "free_count", free_count, 1)
+    if rows < 0:
+        _refuse("kv_plan", "room for %d rows", rows)
+    stream = _here("kv_plan", lens, new_rows, tables, free_blocks, free_count)
     # one piece of memory for everything the plan writes afresh
     sizes = (B + 1, rows, rows, 4, 0 if in_place else B, 0 if in_place else 1, 3 * B + 3)
-    cu, slots, positions, status, out, count, work = torch.empty(sum(sizes), dtype=torch.int32, device=lens.device).split(sizes)
+    cu, slots, positions, status, out, count, work = torch.empty(sum(sizes), dtype=_I32, device=lens.device).split(sizes)
     if in_place:
         out, count = lens, free_count
-    _lib.check(_lib.load().athena_kv_plan(_ptr(lens), _ptr(new_rows), _ptr(tables), ldt, width, _ptr(free_blocks),
-                                          free_blocks.numel(), _ptr(free_count), B, block_size, rows, cu.data_ptr(),
-                                          slots.data_ptr(), positions.data_ptr(), out.data_ptr(), count.data_ptr(),
-                                          status.data_ptr(), work.data_ptr(), _stream()), "athena_kv_plan")
+    _lib.check(_lib.load().athena_kv_plan(_lib.KvPlanDesc.pack(
+        lens.data_ptr(), new_rows.data_ptr(), tables.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), cu.data_ptr(),
+        slots.data_ptr(), positions.data_ptr(), out.data_ptr(), count.data_ptr(), status.data_ptr(), work.data_ptr(),
+        ldt if B > 1 else width, width, free_blocks.numel(), B, block_size, rows, 0), stream), "athena_kv_plan")
     return KvPlan(cu, slots, positions, out, count, status)
 
 
 def _kv8_cache(name, k_codes, v_codes, k_scale, v_scale):
     """(blocks, kv heads, block size, width) of a cache."""
-    if k_codes.dim() != 4 or v_codes.dim() != 4 or k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or \
-            not k_codes.is_contiguous() or not v_codes.is_contiguous():
-        raise RuntimeError("athena_amd.%s: codes must be contiguous int8 [blocks, heads, tokens, columns] (values: columns, "
-                           "tokens)" % name)
-    nb, hk, bs, w = k_codes.shape
-    if tuple(v_codes.shape) != (nb, hk, w, bs):
-        raise RuntimeError("athena_amd.%s: v_codes must be [%d, %d, %d, %d]" % (name, nb, hk, w, bs))
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.numel() != nb * hk or not s.is_contiguous():
-            raise RuntimeError("athena_amd.%s: scales must be contiguous fp32 [%d, %d]" % (name, nb, hk))
+    shape = k_codes.shape
+    if k_codes.dtype is not _I8 or v_codes.dtype is not _I8 or len(shape) != 4 or not k_codes.is_contiguous() or \
+            not v_codes.is_contiguous():
+        _refuse(name, "codes must be contiguous int8 [blocks, heads, tokens, columns] (values: columns, tokens)")
+    nb, hk, bs, w = shape
+    if v_codes.shape != (nb, hk, w, bs):
+        _refuse(name, "v_codes must be [%d, %d, %d, %d]", nb, hk, w, bs)
+    if k_scale.dtype is not _FP32 or v_scale.dtype is not _FP32 or k_scale.shape != (nb, hk) or v_scale.shape != (nb, hk) or \
+            not k_scale.is_contiguous() or not v_scale.is_contiguous():
+        _refuse(name, "scales must be contiguous fp32 [%d, %d]", nb, hk)
     return nb, hk, bs, w
 
 
 def _head_rows(name, what, x):
-    """(row stride, head stride) of [rows, heads, columns] with contiguous columns."""
-    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
-        raise RuntimeError("athena_amd.%s: %s must be [rows, heads, columns] with contiguous columns" % (name, what))
-    return x.stride(0), x.stride(1)
+    """(shape, strides) of [rows, heads, columns] with contiguous columns."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1):
+        _refuse(name, "%s must be [rows, heads, columns] with contiguous columns", what)
+    return shape, stride
 
 
 def kv8_append(k, v, slots, k_codes, v_codes, k_scale, v_scale):
     """Keys and values [rows, kv heads, head size] into the 8-bit cache at ``slots`` [rows] (-1 skips a row);
     see ``athena_kv8_append`` in include/athena_hip.h."""
     nb, hk, bs, w = _kv8_cache("kv8_append", k_codes, v_codes, k_scale, v_scale)
-    ldk, ldk_h = _head_rows("kv8_append", "k", k)
-    ldv, ldv_h = _head_rows("kv8_append", "v", v)
-    n, heads, dk = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype or heads != hk or dk > w:
-        raise RuntimeError("athena_amd.kv8_append: k and v must be alike, [rows, %d, up to %d]" % (hk, w))
-    _ints("kv8_append", slots=(slots, n))
-    _here("kv8_append", k, v, slots, k_codes, v_codes, k_scale, v_scale)
-    _lib.check(_lib.load().athena_kv8_append(_ptr(k), _ptr(v), ldk, ldk_h, ldv, ldv_h, dt(k), _ptr(slots), n, _ptr(k_codes),
-                                             _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), nb, hk, bs, dk, w, _stream()),
-               "athena_kv8_append")
+    shape, sk = _head_rows("kv8_append", "k", k)
+    v_shape, sv = _head_rows("kv8_append", "v", v)
+    n, heads, dk = shape
+    if v_shape != shape or v.dtype != k.dtype or heads != hk or dk > w or dk < 1:
+        _refuse("kv8_append", "k and v must be alike, [rows, %d, up to %d]", hk, w)
+    _int_vector("kv8_append", "slots", slots, n)
+    code = _code("kv8_append", k)
+    stream = _here("kv8_append", k, v, slots, k_codes, v_codes, k_scale, v_scale)
+    _lib.check(_lib.load().athena_kv8_append(_lib.Kv8AppendDesc.pack(
+        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        sk[0], sk[1], sv[0], sv[1], code, n, nb, hk, bs, dk, w, 0), stream), "athena_kv8_append")
 
 
 def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows=None, max_rows=1, causal=True, scale=None,
@@ -1369,49 +1392,64 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows=N
     include/athena_hip.h.  ``cu_rows`` None: row b belongs to sequence b.  ``scale`` None: 1 / sqrt(head size).
     Rows of ``out`` that belong to no sequence are left as they were (not set, without ``out``)."""
     nb, hk, bs, w = _kv8_cache("kv8_attention", k_codes, v_codes, k_scale, v_scale)
-    ldq, ldq_h = _head_rows("kv8_attention", "q", q)
-    n, h, dk = q.shape
+    shape, sq = _head_rows("kv8_attention", "q", q)
+    n, h, dk = shape
     B = lens.numel()
     ldt, width = _tables("kv8_attention", tables, B)
-    if h % hk or dk > w or dk < 1 or max_rows < 1:
-        raise RuntimeError("athena_amd.kv8_attention: %d heads of %d over %d kv heads of up to %d" % (h, dk, hk, w))
+    if h % hk or h < 1 or dk > w or dk < 1 or max_rows < 1:
+        _refuse("kv8_attention", "%d heads of %d over %d kv heads of up to %d, %d rows at most", h, dk, hk, w, max_rows)
+    _int_vector("kv8_attention", "lens", lens, 1)
     if cu_rows is None:
         if n != B:
-            raise RuntimeError("athena_amd.kv8_attention: %d rows for %d sequences need cu_rows" % (n, B))
-        max_rows = 1
-        _ints("kv8_attention", lens=(lens, 1))
+            _refuse("kv8_attention", "%d rows for %d sequences need cu_rows", n, B)
     else:
-        _ints("kv8_attention", lens=(lens, 1), cu_rows=(cu_rows, B + 1))
+        _int_vector("kv8_attention", "cu_rows", cu_rows, B + 1)
     if out is None:
-        out = torch.empty((n, h, dk), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise RuntimeError("athena_amd.kv8_attention: out must be like q")
-    ldo, ldo_h = _head_rows("kv8_attention", "out", out)
-    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n * h or not lse.is_contiguous()):
-        raise RuntimeError("athena_amd.kv8_attention: lse must be contiguous fp32 [%d, %d]" % (n, h))
-    _here("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows, out, lse)
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        so = (h * dk, dk)
+    else:
+        o_shape, so = _head_rows("kv8_attention", "out", out)
+        if o_shape != shape or out.dtype != q.dtype:
+            _refuse("kv8_attention", "out must be like q")
+    if lse is not None and (lse.dtype is not _FP32 or lse.numel() != n * h or not lse.is_contiguous()):
+        _refuse("kv8_attention", "lse must be contiguous fp32 [%d, %d]", n, h)
+    code = _code("kv8_attention", q)
+    stream = _here("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows, out, lse)
     lib = _lib.load()
-    need = lib.athena_kv8_attention_workspace_bytes(dt(q), B, max_rows, n, h, hk, width, bs, dk, w)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.check(lib.athena_kv8_attention(_ptr(q), ldq, ldq_h, dt(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale),
-                                        nb, bs, w, _ptr(tables), ldt, width, _ptr(lens), _ptr(cu_rows), B, max_rows, n, h, hk,
-                                        dk, 1 if causal else 0, scale if scale is not None else 1.0 / math.sqrt(dk),
-                                        out.data_ptr(), ldo, ldo_h, _ptr(lse), _ptr(ws), need, _stream()),
-               "athena_kv8_attention")
+    work = 0
+    while True:
+        desc = _lib.Kv8AttentionDesc.pack(
+            q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), tables.data_ptr(),
+            lens.data_ptr(), cu_rows.data_ptr() if cu_rows is not None else 0, out.data_ptr(),
+            lse.data_ptr() if lse is not None else 0, ws.data_ptr() if work else 0, work, sq[0], sq[1], so[0], so[1], ldt, code, nb, bs, w,
+            width, B, max_rows, n, h, hk, dk, 1 if causal else 0, scale if scale is not None else 1.0 / math.sqrt(dk), 0.0)
+        # (a table of fewer than 2048 places never needs a workspace)
+        if work or width * bs < 2048:
+            break
+        work = lib.athena_kv8_attention_workspace_bytes(desc)
+        if not work:
+            break
+        ws = torch.empty(work, dtype=torch.uint8, device=q.device)
+    _lib.check(lib.athena_kv8_attention(desc, stream), "athena_kv8_attention")
     return out
 
 
 def _row_vector(name, what, t, rows):
-    if t is not None and (t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous()):
-        raise RuntimeError("athena_amd.%s: %s must be contiguous fp32 [%d]" % (name, what, rows))
+    if t is None:
+        return 0
+    if t.dtype is not _FP32 or t.numel() != rows or not t.is_contiguous():
+        _refuse(name, "%s must be contiguous fp32 [%d]", what, rows)
+    return t.data_ptr()
 
 
 def _row_matrix(name, what, t, dtype, rows, cols):
     """Leading dimension of [rows, cols], or 0 for one row [cols] / [1, cols] that serves all."""
-    if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] != cols or (cols > 1 and t.stride(-1) != 1) or \
-            (t.dim() == 2 and t.shape[0] not in (1, rows)):
-        raise RuntimeError("athena_amd.%s: %s must be %s [%d, %d] or one such row" % (name, what, dtype, rows, cols))
-    return t.stride(0) if t.dim() == 2 and t.shape[0] == rows else 0
+    shape, stride = t.shape, t.stride()
+    dims = len(shape)
+    if t.dtype is not dtype or dims not in (1, 2) or shape[-1] != cols or (stride[-1] != 1 and cols > 1) or \
+            (dims == 2 and shape[0] != rows and shape[0] != 1):
+        _refuse(name, "%s must be %s [%d, %d] or one such row", what, dtype, rows, cols)
+    return stride[0] if dims == 2 and shape[0] == rows else 0
 
 
 def logits_process(logits, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
@@ -1421,40 +1459,45 @@ def logits_process(logits, history=None, history_len=None, repetition=None, pres
     [rows]; ``repetition``, ``presence``, ``frequency`` fp32 [rows]; ``bias`` fp32 [rows or 1, classes];
     ``bias_ids`` / ``bias_values`` int32 / fp32 [rows, n]; ``allowed`` int32 [rows or 1, ceil(classes / 32)], a bit per
     class.  Returns ``out`` (a new tensor unless given; it may be ``logits``)."""
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise RuntimeError("athena_amd.logits_process: logits must be [rows, classes] with contiguous rows")
-    R, V = logits.shape
+    name = "logits_process"
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+        _refuse(name, "logits must be [rows, classes] with contiguous rows")
+    R, V = shape
     L = ldh = ldb = ldi = ldv = lda = nb = 0
     if history is not None:
         L = history.shape[-1]
+        ldh = _row_matrix(name, "history", history, _I32, R, L)
         if history.dim() != 2 or history.shape[0] != R:
-            raise RuntimeError("athena_amd.logits_process: history must be int32 [%d, tokens]" % R)
-        ldh = _row_matrix("logits_process", "history", history, torch.int32, R, L)
+            _refuse(name, "history must be int32 [%d, tokens]", R)
         if history_len is not None:
-            _ints("logits_process", history_len=(history_len, R))
+            _int_vector(name, "history_len", history_len, R)
     elif history_len is not None or repetition is not None or presence is not None or frequency is not None:
-        raise RuntimeError("athena_amd.logits_process: penalties need a history")
-    _row_vector("logits_process", "repetition", repetition, R)
-    _row_vector("logits_process", "presence", presence, R)
-    _row_vector("logits_process", "frequency", frequency, R)
+        _refuse(name, "penalties need a history")
+    rep, pres, freq = _row_vector(name, "repetition", repetition, R), _row_vector(name, "presence", presence, R), \
+        _row_vector(name, "frequency", frequency, R)
     if bias is not None:
-        ldb = _row_matrix("logits_process", "bias", bias, torch.float32, R, V)
+        ldb = _row_matrix(name, "bias", bias, _FP32, R, V)
     if (bias_ids is None) != (bias_values is None):
-        raise RuntimeError("athena_amd.logits_process: bias_ids and bias_values come together")
+        _refuse(name, "bias_ids and bias_values come together")
     if bias_ids is not None:
         nb = bias_ids.shape[-1]
-        ldi = _row_matrix("logits_process", "bias_ids", bias_ids, torch.int32, R, nb)
-        ldv = _row_matrix("logits_process", "bias_values", bias_values, torch.float32, R, nb)
+        ldi = _row_matrix(name, "bias_ids", bias_ids, _I32, R, nb)
+        ldv = _row_matrix(name, "bias_values", bias_values, _FP32, R, nb)
     if allowed is not None:
-        lda = _row_matrix("logits_process", "allowed", allowed, torch.int32, R, (V + 31) // 32)
+        lda = _row_matrix(name, "allowed", allowed, _I32, R, (V + 31) // 32)
     if out is None:
-        out = torch.empty((R, V), dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1):
-        raise RuntimeError("athena_amd.logits_process: out must be like logits")
-    _here("logits_process", logits, history, history_len, repetition, presence, frequency, bias, bias_ids, bias_values, allowed,
-          out)
-    _lib.check(_lib.load().athena_logits_process(
-        _ptr(logits), logits.stride(0) if R > 1 else V, dt(logits), R, V, _ptr(history), ldh, L, _ptr(history_len), _ptr(repetition),
-        _ptr(presence), _ptr(frequency), _ptr(bias), ldb, _ptr(bias_ids), ldi, _ptr(bias_values), ldv, nb, _ptr(allowed), lda,
-        out.data_ptr(), out.stride(0) if R > 1 else V, _stream()), "athena_logits_process")
+        out, ldo = torch.empty(shape, dtype=logits.dtype, device=logits.device), V
+    else:
+        so = out.stride()
+        if out.shape != shape or out.dtype != logits.dtype or (so[1] != 1 and V > 1):
+            _refuse(name, "out must be like logits")
+        ldo = so[0] if R > 1 else V
+    code = _code(name, logits)
+    stream = _here(name, logits, history, history_len, repetition, presence, frequency, bias, bias_ids, bias_values, allowed, out)
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    _lib.check(_lib.load().athena_logits_process(_lib.LogitsDesc.pack(
+        logits.data_ptr(), out.data_ptr(), ptr(history), ptr(history_len), ptr(bias_ids), ptr(allowed), rep, pres, freq, ptr(bias),
+        ptr(bias_values), stride[0] if R > 1 else V, ldo, ldh, ldb, ldi, ldv, lda, code, R, V, L, nb, 0), stream),
+        "athena_logits_process")
     return out

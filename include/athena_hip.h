@@ -771,10 +771,15 @@ int athena_copy_many(const void* const* src, void* const* dst, const long* bytes
  * free_capacity}.  A plan that does not fit leaves a status that is not zero and changes nothing: no rows
  * (cu_rows 0, slots -1), lens_out = lens, free_count_out = free_count.  ``work``: int32 [3 * B + 3].
  * A block belongs to one request. */
-int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int32_t* tables, long ld_tables, int table_width,
-                   int32_t* free_blocks, int free_capacity, const int32_t* free_count, int B, int block_size, int rows,
-                   int32_t* cu_rows, int32_t* slots, int32_t* positions, int32_t* lens_out, int32_t* free_count_out,
-                   int32_t* status, int32_t* work, athena_stream_t stream);
+typedef struct {
+    const int32_t *lens, *new_rows;
+    int32_t *tables, *free_blocks;
+    const int32_t* free_count;
+    int32_t *cu_rows, *slots, *positions, *lens_out, *free_count_out, *status, *work;
+    int64_t ld_tables;
+    int32_t table_width, free_capacity, B, block_size, rows, reserved;
+} athena_kv_plan_desc;
+int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stream);
 
 /* Keys and values of N rows into their places.  Row t: k[t * ldk + head * ldk_head + c], c < dk; a slot
  * outside [0, num_blocks * block_size) skips its row.  Rows of one block stand one behind the other (as
@@ -784,9 +789,15 @@ int athena_kv_plan(const int32_t* lens, const int32_t* new_rows, int32_t* tables
  * the grown scale (round half to even of code * old / new); a run that begins at a block's first place
  * begins the block again, whatever its scale was.  Codes are round half to even of x / scale.  A value that
  * is not finite makes its block's scale NaN: the block then stands for NaN until it is begun again. */
-int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, long ldv, long ldv_head, int dtype,
-                      const int32_t* slots, int N, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
-                      int num_blocks, int hk, int block_size, int dk, int width, athena_stream_t stream);
+typedef struct {
+    const void *k, *v;
+    const int32_t* slots;
+    int8_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    int64_t ldk, ldk_head, ldv, ldv_head;
+    int32_t dtype, N, num_blocks, hk, block_size, dk, width, reserved;
+} athena_kv8_append_desc;
+int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_t stream);
 
 /* Attention over the cache: out[t, head] = sum_j softmax_j(scale * q[t, head] . k_j) v_j over the cached
  * tokens of t's sequence.  Sequence b has lens[b] tokens (its new ones included) and the query rows
@@ -797,15 +808,22 @@ int athena_kv8_append(const void* k, const void* v, long ldk, long ldk_head, lon
  * max_rows: the largest number of rows of a sequence (it shapes the launch; results do not depend on it).
  * lse: fp32 [N][h], natural logarithm of the sum of exponentials, or null.
  * ld_tables may be 0: every sequence then reads the same blocks.
- * ``workspace``: athena_kv8_attention_workspace_bytes (0: none is needed). */
-int64_t athena_kv8_attention_workspace_bytes(int dtype, int B, int max_rows, int N, int h, int hk, int table_width,
-                                             int block_size, int dk, int width);
-int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, const int8_t* k_codes, const int8_t* v_codes,
-                         const float* k_scale, const float* v_scale, int num_blocks, int block_size, int width,
-                         const int32_t* tables, long ld_tables, int table_width, const int32_t* lens,
-                         const int32_t* cu_rows, int B, int max_rows, int N, int h, int hk, int dk, int causal,
-                         float scale, void* out, long ldo, long ldo_head, float* lse, void* workspace,
-                         int64_t workspace_bytes, athena_stream_t stream);
+ * ``workspace``: athena_kv8_attention_workspace_bytes of the same descriptor (0: none is needed; its pointers are
+ * not looked at, and a table of fewer than 2048 places never needs one). */
+typedef struct {
+    const void* q;
+    const int8_t *k_codes, *v_codes;
+    const float *k_scale, *v_scale;
+    const int32_t *tables, *lens, *cu_rows;
+    void* out;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes, ldq, ldq_head, ldo, ldo_head, ld_tables;
+    int32_t dtype, num_blocks, block_size, width, table_width, B, max_rows, N, h, hk, dk, causal;
+    float scale, reserved;
+} athena_kv8_attention_desc;
+int64_t athena_kv8_attention_workspace_bytes(const athena_kv8_attention_desc* d);
+int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_stream_t stream);
 
 /* Penalties, biases and a grammar mask on the logits of a decoding step, between the output layer and the
  * search (the reference adds scorers to log-probabilities on the host, athena/tools/beam_search.py:120-150).
@@ -816,11 +834,15 @@ int athena_kv8_attention(const void* q, long ldq, long ldq_head, int dtype, cons
  *   -inf unless bit v % 32 of word v / 32 of allowed[r * ld_allowed + ...] is set.
  * Any of history, repetition, presence, frequency, bias, bias_ids (nb = 0), allowed may be null.  ld_bias and
  * ld_allowed may be 0 (one row for all).  out has the type of the logits and may be the logits. */
-int athena_logits_process(const void* logits, long ldl, int dtype, int R, int V, const int32_t* history, long ld_history,
-                          int L, const int32_t* history_len, const float* repetition, const float* presence,
-                          const float* frequency, const float* bias, long ld_bias, const int32_t* bias_ids,
-                          long ld_bias_ids, const float* bias_values, long ld_bias_values, int nb,
-                          const int32_t* allowed, long ld_allowed, void* out, long ldo, athena_stream_t stream);
+typedef struct {
+    const void* logits;
+    void* out;
+    const int32_t *history, *history_len, *bias_ids, *allowed;
+    const float *repetition, *presence, *frequency, *bias, *bias_values;
+    int64_t ldl, ldo, ld_history, ld_bias, ld_bias_ids, ld_bias_values, ld_allowed;
+    int32_t dtype, R, V, L, nb, reserved;
+} athena_logits_desc;
+int athena_logits_process(const athena_logits_desc* d, athena_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,5 @@
 """What the decoding operators refuse, checked in front of any launch (no GPU is needed), and the loop
 restatements the GPU tests compare with, checked against hand-made cases."""
-import ctypes
-
 import pytest
 import torch
 
@@ -92,26 +90,28 @@ def test_logits_refusals(change):
 
 
 def test_the_c_entries_refuse_before_any_launch():
-    lib, p = _lib.load(), ctypes.c_void_p(4096)         # an address that is never followed
-    attn = lambda bs=16, w=32, h=4, dk=32, dtype=0, q=p, nb=4, B=1, mr=1, codes=p: lib.athena_kv8_attention(
-        q, 128, 32, dtype, codes, p, p, p, nb, bs, w, p, 1, 1, p, None, B, mr, 1, h, 2, dk, 1, 1.0, p, 128, 32, None, None, 0, None)
-    for kw in (dict(bs=24), dict(w=48), dict(h=3), dict(dk=33), dict(dk=0), dict(dtype=2), dict(q=None), dict(nb=0), dict(B=0),
-               dict(B=70000), dict(mr=0), dict(nb=1 << 28), dict(codes=ctypes.c_void_p(4100))):
+    lib, p = _lib.load(), 4096                          # an address that is never followed
+    attn = lambda bs=16, w=32, h=4, dk=32, dtype=0, q=p, nb=4, B=1, n=1, cu=0, mr=1, codes=p, W=1, ws=0: lib.athena_kv8_attention(
+        _lib.Kv8AttentionDesc.pack(q, codes, p, p, p, p, p, cu, p, 0, ws, 0, 128, 32, 128, 32, W, dtype, nb, bs, w, W, B, mr, n, h, 2, dk, 1,
+                                   1.0, 0.0), None)
+    for kw in (dict(bs=24), dict(w=48), dict(h=3), dict(dk=33), dict(dk=0), dict(dtype=2), dict(q=0), dict(nb=0), dict(B=0),
+               dict(B=70000), dict(cu=p, mr=0), dict(nb=1 << 28), dict(codes=4100), dict(n=2), dict(W=1 << 20), dict(W=1 << 27)):
         assert attn(**kw) < 0, kw
         assert b"athena_kv8_attention" in lib.athena_last_error()
+    assert lib.athena_kv8_attention(None, None) < 0 and lib.athena_kv8_attention_workspace_bytes(None) == 0
     append = lambda bs=16, w=32, dk=32, dtype=0, k=p, n=1, codes=p: lib.athena_kv8_append(
-        k, p, 64, 32, 64, 32, dtype, p, n, codes, p, p, p, 4, 2, bs, dk, w, None)
-    for kw in (dict(bs=8), dict(w=256), dict(dk=64), dict(dtype=5), dict(k=None), dict(n=-1), dict(codes=ctypes.c_void_p(4097))):
+        _lib.Kv8AppendDesc.pack(k, p, p, codes, p, p, p, 64, 32, 64, 32, dtype, n, 4, 2, bs, dk, w, 0), None)
+    for kw in (dict(bs=8), dict(w=256), dict(dk=64), dict(dtype=5), dict(k=0), dict(n=-1), dict(codes=4097)):
         assert append(**kw) < 0, kw
         assert b"athena_kv8_append" in lib.athena_last_error()
     plan = lambda B=1, W=4, ld=4, free=4, bs=16, rows=1, lens=p: lib.athena_kv_plan(
-        lens, p, p, ld, W, p, free, p, B, bs, rows, p, p, p, p, p, p, p, None)
-    for kw in (dict(B=0), dict(W=0), dict(ld=3), dict(free=0), dict(bs=20), dict(rows=-1), dict(lens=None), dict(W=1 << 27, ld=1 << 27)):
+        _lib.KvPlanDesc.pack(lens, p, p, p, p, p, p, p, p, p, p, p, ld, W, free, B, bs, rows, 0), None)
+    for kw in (dict(B=0), dict(W=0), dict(ld=3), dict(free=0), dict(bs=20), dict(rows=-1), dict(lens=0), dict(W=1 << 27, ld=1 << 27)):
         assert plan(**kw) < 0, kw
         assert b"athena_kv_plan" in lib.athena_last_error()
     logits = lambda R=1, V=40, ldl=40, dtype=0, x=p, nb=0: lib.athena_logits_process(
-        x, ldl, dtype, R, V, None, 0, 0, None, None, None, None, None, 0, None, 0, None, 0, nb, None, 0, p, 40, None)
-    for kw in (dict(R=-1), dict(V=0), dict(ldl=39), dict(dtype=3), dict(x=None), dict(nb=1), dict(R=70000)):
+        _lib.LogitsDesc.pack(x, p, 0, 0, 0, 0, 0, 0, 0, 0, 0, ldl, 40, 0, 0, 0, 0, 0, dtype, R, V, 0, nb, 0), None)
+    for kw in (dict(R=-1), dict(V=0), dict(ldl=39), dict(dtype=3), dict(x=0), dict(nb=1), dict(R=70000)):
         assert logits(**kw) < 0, kw
         assert b"athena_logits_process" in lib.athena_last_error()
     assert logits(R=0) == 0 and append(n=0) == 0
