@@ -362,36 +362,45 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
     }
 }
 
-// out = the splits' results weighted by their share of the sum of exponentials; one wave per (row, head)
+// out = the splits' results weighted by their share of the sum of exponentials; one wave per (row, head).  Bound by the
+// latency of its loads: the weights are worked out by the lanes side by side, the results then requested eight at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttn a) {
     const int lane = threadIdx.x & 63, head = blockIdx.y * 4 + (threadIdx.x >> 6), b = blockIdx.z;
     if (head >= a.h) return;
     const int lo = min(max(a.cu_rows ? a.cu_rows[b] : b, 0), a.N), hi = min(max(a.cu_rows ? a.cu_rows[b + 1] : b + 1, lo), a.N);
+    const int c0 = lane < a.dk ? lane : 0, c1 = lane + 64 < a.dk ? lane + 64 : c0;
     for (long t = lo + blockIdx.x; t < hi; t += gridDim.x) {
         const long at = t * a.h + head, step = (long)a.N * a.h;
         float top = -INFINITY;
-        for (int i = lane; i < a.splits; i += 64) {
-            const float x = a.part_lse[at + i * step];
-            top = fmaxf(top, x);
-        }
+        for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, a.part_lse[at + i * step]);
         top = wave_max(top);
         const float base = top == -INFINITY ? 0.f : top;
-        float o[2] = {0.f, 0.f}, sum = 0.f;
-        for (int i = 0; i < a.splits; ++i) {
-            const float x = a.part_lse[at + i * step];
-            if (x == -INFINITY) continue;
-            const float weight = __builtin_amdgcn_exp2f(x - base);
-            sum += weight;
+        float o0 = 0.f, o1 = 0.f, sum = 0.f;
+        for (int i0 = 0; i0 < a.splits; i0 += 64) {
+            const float mine = i0 + lane < a.splits ? __builtin_amdgcn_exp2f(a.part_lse[at + (i0 + lane) * step] - base) : 0.f;
+            sum += mine;
+            for (int i = 0; i < 64 && i0 + i < a.splits; i += 8) {
+                float x0[8], x1[8];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (lane + 64 * j < a.dk) o[j] += weight * a.part[(at + i * step) * a.dk + lane + 64 * j];
+                for (int j = 0; j < 8; ++j) {
+                    const float* p = a.part + (at + (long)min(i0 + i + j, a.splits - 1) * step) * a.dk;
+                    x0[j] = p[c0];
+                    x1[j] = p[c1];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float weight = __shfl(mine, i + j, 64);       // 0: a split without tokens leaves no result
+                    o0 += weight != 0.f ? weight * x0[j] : 0.f;
+                    o1 += weight != 0.f ? weight * x1[j] : 0.f;
+                }
+            }
         }
+        sum = wave_sum(sum);
         const float inv = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
         T* out = (T*)a.out + t * a.ldo + (long)head * a.ldo_head;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (lane + 64 * j < a.dk) out[lane + 64 * j] = from_f32<T>(o[j] * inv);
+        if (lane < a.dk) out[lane] = from_f32<T>(o0 * inv);
+        if (lane + 64 < a.dk) out[lane + 64] = from_f32<T>(o1 * inv);
         if (a.lse && lane == 0)
             a.lse[at] = sum > 0.f ? (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : sum != sum ? sum : -INFINITY;
     }

@@ -39,10 +39,10 @@ __device__ __forceinline__ long long shfl_up64(long long v, int o) { return __sh
 // blocks of n tokens
 __device__ __forceinline__ int blocks_of(long long n, int bs) { return (int)((n + bs - 1) / bs); }
 
-__device__ __forceinline__ int plan_stack(const PlanArgs& a, int count, int at) {
-    // entry ``at`` of the stack of free blocks with the given-back ones on top of it
+// entry ``at`` of the stack of free blocks with the given-back ones on top of it; ``given`` [B]: given-back blocks in front
+// of a request (in LDS where they fit)
+__device__ __forceinline__ int plan_stack(const PlanArgs& a, const int32_t* given, int count, int at) {
     if (at < count) return a.free_blocks[at];
-    const int32_t* given = a.work + a.B;
     const int f = at - count;
     int lo = 0, hi = a.B - 1;                   // last request whose first given-back block is <= f
     while (lo < hi) {
@@ -53,42 +53,43 @@ __device__ __forceinline__ int plan_stack(const PlanArgs& a, int count, int at) 
     return a.tables[(long)lo * a.ld_tables + (f - given[lo])];
 }
 
-// threads [first, first + step, ...) of the rows, waves [first / 64, ...) of the requests
-__device__ __forceinline__ void plan_fill(const PlanArgs& a, int first, int step) {
+// a wave per request: its rows, its new table entries or its returned blocks; threads [first, first + step, ...)
+__device__ __forceinline__ void plan_fill(const PlanArgs& a, const int32_t* given, int first, int step) {
     const int32_t* end = a.work + 2 * a.B;
-    const int count = end[0], level = end[1], fits = end[2];
-    const int total = fits ? a.cu_rows[a.B] : 0;
-    for (int t = first; t < a.rows; t += step) {
-        int slot = -1, pos = 0;
-        if (t < total) {
-            int lo = 0, hi = a.B - 1;           // last request that begins at or before row t
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (a.cu_rows[mid] <= t) lo = mid;
-                else hi = mid - 1;
-            }
-            const int len = a.before[lo];
-            pos = len + t - a.cu_rows[lo];
-            const int j = pos / a.block_size, have = blocks_of(len, a.block_size);
-            const int block = j < have ? a.tables[(long)lo * a.ld_tables + j]
-                                       : plan_stack(a, count, level - 1 - (a.work[lo] + j - have));
-            slot = block < 0 ? -1 : block * a.block_size + pos % a.block_size;
-        }
-        a.slots[t] = slot;
-        a.positions[t] = pos;
+    const int count = end[0], level = end[1], fits = end[2], bs = a.block_size;
+    for (int t = (fits ? a.cu_rows[a.B] : 0) + first; t < a.rows; t += step) {      // behind the last row
+        a.slots[t] = -1;
+        a.positions[t] = 0;
     }
     if (!fits) return;
     const int lane = first & 63;
     for (int b = first >> 6; b < a.B; b += step >> 6) {
-        const int len = a.before[b], n = a.new_rows[b];
-        const int have = blocks_of(len, a.block_size);
+        const int len = a.before[b], n = a.new_rows[b], have = blocks_of(len, bs);
         int32_t* row = a.tables + (long)b * a.ld_tables;
         if (n < 0) {
             const int at = count + a.work[a.B + b];
             for (int j = lane; j < have; j += 64) a.free_blocks[at + j] = row[j];
-        } else {
-            const int need = blocks_of((long long)len + n, a.block_size) - have;
-            for (int j = lane; j < need; j += 64) row[have + j] = plan_stack(a, count, level - 1 - (a.work[b] + j));
+            continue;
+        }
+        const int row0 = a.cu_rows[b], taken = a.work[b];
+        // 64 blocks at a time: a lane finds one of them, then the rows look their block up in the lanes
+        const int last = blocks_of((long long)len + n, bs);
+        for (int j0 = len / bs; j0 < last; j0 += 64) {
+            const int j = j0 + lane;
+            int block = -1;
+            if (j < have) block = row[j];
+            else if (j < last) {
+                block = plan_stack(a, given, count, level - 1 - (taken + j - have));
+                row[j] = block;
+            }
+            const int from = max(j0 * bs, len), to = (int)min((long long)(j0 + 64) * bs, (long long)len + n);
+            for (int p0 = from; p0 < to; p0 += 64) {
+                const int p = p0 + lane, mine = __shfl(block, min(p / bs - j0, 63), 64);
+                if (p < to) {
+                    a.slots[row0 + p - len] = mine < 0 ? -1 : mine * bs + p % bs;
+                    a.positions[row0 + p - len] = p;
+                }
+            }
         }
     }
 }
@@ -172,11 +173,19 @@ __global__ __launch_bounds__(PLAN_THREADS) void kv_plan_kernel(PlanArgs a, int f
     if (!fill) return;
     __threadfence_block();
     __syncthreads();
-    plan_fill(a, tid, PLAN_THREADS);
+    plan_fill(a, a.work + a.B, tid, PLAN_THREADS);
 }
 
+#define PLAN_LDS 8192       // requests whose running sums a workgroup keeps in LDS
 __global__ __launch_bounds__(256) void kv_plan_fill_kernel(PlanArgs a) {
-    plan_fill(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    __shared__ int32_t sums[PLAN_LDS];
+    const int32_t* given = a.work + a.B;
+    if (a.B <= PLAN_LDS) {
+        for (int b = threadIdx.x; b < a.B; b += 256) sums[b] = given[b];
+        __syncthreads();
+        given = sums;
+    }
+    plan_fill(a, given, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 extern "C" int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stream) {
@@ -195,13 +204,13 @@ extern "C" int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stre
                   d->lens_out, d->free_count_out, d->status, d->work, d->work + 2L * d->B + 3, d->B, d->table_width,
                   d->free_capacity, bs, d->rows};
     hipStream_t s = (hipStream_t)stream;
-    // one workgroup fills up to four rows a thread and 16 requests a wave itself; beyond that a launch of many is faster
-    const int fill = d->rows <= 4 * PLAN_THREADS && d->B <= 16 * (PLAN_THREADS / 64);
+    // one workgroup fills the rows of a few requests a wave itself; beyond that a launch of many is faster
+    const int fill = d->rows <= 4 * PLAN_THREADS && d->B <= 8 * (PLAN_THREADS / 64);
     ATHENA_LAUNCH(kv_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, s, a, fill);
     ATHENA_CHECK_LAUNCH("athena_kv_plan");
     if (!fill) {
-        const long units = (long)d->B * 64 > d->rows ? (long)d->B * 64 : d->rows, wgs = (units + 255) / 256;
-        ATHENA_LAUNCH(kv_plan_fill_kernel, dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, s, a);
+        const int wgs = (d->B + 3) / 4;
+        ATHENA_LAUNCH(kv_plan_fill_kernel, dim3(wgs < 1024 ? wgs : 1024), dim3(256), 0, s, a);
         ATHENA_CHECK_LAUNCH("athena_kv_plan (fill)");
     }
     return ATHENA_OK;
@@ -260,23 +269,29 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, bool values, 
     int8_t* codes = a.codes + at * W * block_size;
     const int step = 16 * SUB, begin = first & ~15, end = first + n;
     float v[16][2];
-    auto load = [&](int base) {                             // the two columns of places base + 16 sub ...
+    struct alignas(2 * sizeof(T)) Pair { T e[2]; };
+    // the two columns of places base + 16 sub ...: all sixteen requests go out before the first is waited for, so rows and
+    // columns that are not there are read from ones that are, and dropped afterwards
+    auto load = [&](int base) {
         const int p0 = base + 16 * sub;
+        const int c0 = c < dk ? c : 0, c1 = c + 1 < dk ? c + 1 : 0;
+        Pair raw[16];
+        if (pairs && (dk & 1) == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) raw[i] = *(const Pair*)(x + (long)min(max(p0 + i - first, 0), n - 1) * a.ld_row + c0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const T* p = x + (long)min(max(p0 + i - first, 0), n - 1) * a.ld_row;
+                raw[i].e[0] = p[c0];
+                raw[i].e[1] = p[c1];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            v[i][0] = v[i][1] = 0.f;
-            if (p0 + i >= first && p0 + i < end && c < dk) {
-                const T* p = x + (long)(p0 + i - first) * a.ld_row + c;
-                if (pairs && c + 1 < dk) {
-                    struct alignas(2 * sizeof(T)) Pair { T e[2]; };
-                    const Pair two = *(const Pair*)p;
-                    v[i][0] = to_f32<T>(two.e[0]);
-                    v[i][1] = to_f32<T>(two.e[1]);
-                } else {
-                    v[i][0] = to_f32<T>(p[0]);
-                    if (c + 1 < dk) v[i][1] = to_f32<T>(p[1]);
-                }
-            }
+            const bool in = p0 + i >= first && p0 + i < end;
+            v[i][0] = in && c < dk ? to_f32<T>(raw[i].e[0]) : 0.f;
+            v[i][1] = in && c + 1 < dk ? to_f32<T>(raw[i].e[1]) : 0.f;
         }
     };
     unsigned top = 0;                                       // largest magnitude, as bits: NaN over infinity over numbers

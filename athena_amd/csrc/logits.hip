@@ -19,12 +19,16 @@ struct LogitsArgs {
 };
 
 #define LOGITS_BIASED 0x80000000u
+#define LOGITS_LIST 256         // biases of one tile kept in LDS; more are looked up in memory
 
 // NB vectors of 16 bytes per thread
 template <typename T, int NB>
 __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
     constexpr int E = 16 / sizeof(T), TILE = 256 * E * NB;
     __shared__ __attribute__((aligned(16))) unsigned count[TILE];
+    __shared__ unsigned list_at[LOGITS_LIST];
+    __shared__ float list_value[LOGITS_LIST];
+    __shared__ int listed;
     struct alignas(16) Vec { T e[E]; };
     const int r = blockIdx.y, v0 = blockIdx.x * TILE, nv = min(TILE, a.V - v0), tid = threadIdx.x;
     const T* in = (const T*)a.logits + (long)r * a.ldl + v0;
@@ -53,11 +57,26 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
             if (at < (unsigned)nv) atomicAdd(&count[at], 1u);
         }
     }
-    for (int j = tid; j < a.nb; j += 256) {
-        const unsigned at = (unsigned)a.bias_ids[(long)r * a.ld_bias_ids + j] - (unsigned)v0;
-        if (at < (unsigned)nv) atomicOr(&count[at], LOGITS_BIASED);
+    if (tid < 64) {                             // the tile's own biases, in their order
+        int n = 0;
+        for (int j0 = 0; j0 < a.nb; j0 += 64) {
+            const int j = j0 + tid;
+            const unsigned at = j < a.nb ? (unsigned)a.bias_ids[(long)r * a.ld_bias_ids + j] - (unsigned)v0 : ~0u;
+            const unsigned long long found = __ballot(at < (unsigned)nv);
+            if (at < (unsigned)nv) {
+                atomicOr(&count[at], LOGITS_BIASED);
+                const int k = n + __popcll(found & ((1ull << tid) - 1));
+                if (k < LOGITS_LIST) {
+                    list_at[k] = at;
+                    list_value[k] = a.bias_values[(long)r * a.ld_bias_values + j];
+                }
+            }
+            n += __popcll(found);
+        }
+        if (tid == 0) listed = n;
     }
     __syncthreads();
+    const int biased = listed;
     const float rep = a.repetition ? a.repetition[r] : 1.f, pres = a.presence ? a.presence[r] : 0.f,
                 freq = a.frequency ? a.frequency[r] : 0.f;
 #pragma unroll
@@ -76,8 +95,12 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
             if (a.bias && i + e < nv) y += a.bias[(long)r * a.ld_bias + v];
             if (c & LOGITS_BIASED) {
                 float own = 0.f;                // entries of one class add up in their order
-                for (int j = 0; j < a.nb; ++j)
-                    if (a.bias_ids[(long)r * a.ld_bias_ids + j] == v) own += a.bias_values[(long)r * a.ld_bias_values + j];
+                if (biased <= LOGITS_LIST) {
+                    for (int j = 0; j < biased; ++j) own += list_at[j] == (unsigned)(i + e) ? list_value[j] : 0.f;
+                } else {
+                    for (int j = 0; j < a.nb; ++j)
+                        if (a.bias_ids[(long)r * a.ld_bias_ids + j] == v) own += a.bias_values[(long)r * a.ld_bias_values + j];
+                }
                 y += own;
             }
             x[b].e[e] = from_f32<T>((mask[b] >> (v & 31)) & 1u ? y : -INFINITY);
