@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
     constexpr int F = W / 32, D = W / 16, ROWS = 16 * RT;
     __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_m2[4][ROWS];
     __shared__ float s_o[4][ROWS][W + 4];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, qc = lane & 15;
+    // (what is the same in all lanes of a wave is said to be, or the compiler keeps it per lane)
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, qc = lane & 15;
     // workgroups of one (sequence, kv head) lie eight apart, on one XCD: they share its L2
     const int inner = a.row_tiles * a.splits, unit = blockIdx.x / 8;
     const int pair = unit / inner * 8 + blockIdx.x % 8, part = unit % inner;
@@ -149,6 +150,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
             least = min(least, __shfl_xor(least, o, 64));
             most = max(most, __shfl_xor(most, o, 64));
         }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
         // ---- this workgroup's tiles of keys
         const int tiles = (most + KV_KEYS - 1) / KV_KEYS;
         const int per = a.splits > 1 ? max((tiles + a.splits - 1) / a.splits, KV_MIN_TILES) : tiles;

@@ -219,16 +219,17 @@ extern "C" int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stre
 // ---------------------------------------------------------------- writing new keys and values
 // Consecutive rows that go to the same block are one run: the block's scale grows to the largest magnitude of
 // the run / 127 (from nothing where the run begins the block), codes in front of the run are brought to a grown
-// scale, and the run's codes are written.  One wave per (run, kv head, keys or values); the wave that finds a
-// run's first row takes all of it, so waves of one block never meet.
+// scale, and the run's codes are written.  A run, kv head and side (keys or values) belongs to one wave, or to a
+// team of four that divide its places and exchange their largest magnitudes; the workgroup that finds a run's first
+// row takes all of it, so two never meet in a block.
 //
-// Codes are round-half-to-even(x / scale) exactly: the product with the reciprocal in fp32 is off by less
-// than 127 * 2^-23, so a quotient within 1e-4 of a border is divided again in 64 bits, where quotients of
-// fp32 operands of this size cannot come closer than 2^-34 to a border without lying on it.
+// Codes are round-half-to-even(x / scale) exactly.  (bf16 values and a scale made of one of them have few distinct
+// quotients: one in 300 lies on or next to a border.)  The quotient in fp32 gives a whole number next to the right one,
+// and the remainder x - code * scale, which one fused multiply-add leaves exactly (a multiple of 2^-24 of the scale's power
+// of two, at most half the scale or so), decides.  Rounding in fp32 is an addition of 1.5 * 2^23, whose lowest byte is the code.
 //
 // A lane holds two columns of 16 consecutive places, so that the values' codes (16 bytes of one column) leave
-// in one store.  Bound by the rows' way in and the codes' way out; a run of more places than the wave holds at
-// once reads its rows twice, the second time from the caches.
+// in one store.  Bound by the rows' way in and the codes' way out.
 template <typename T> struct AppendSide {
     const T* x;
     long ld_row, ld_head;
@@ -236,73 +237,100 @@ template <typename T> struct AppendSide {
     float* scale;
 };
 
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
-    const float f = x * inv;
-    float q = rintf(f);
-    if (fabsf(fabsf(f - q) - 0.5f) < 1e-4f || s < 1e-30f) q = s > 0.f ? (float)rint((double)x / (double)s) : 0.f;
-    return (int)fminf(fmaxf(q, -127.f), 127.f);
+#define KV_ROUND 12582912.f         // 1.5 * 2^23
+#define KV_DOUBT 1.3e-7f            // a product in fp32 of a rounded ratio is off by at most 2^-23 of itself
+// code of a number, in the lowest byte; ``s`` at least 1e-30 (see tiny below)
+__device__ __forceinline__ unsigned code_of(float x, float s, float inv) {
+    const float y = fmaf(x, inv, KV_ROUND), r = fmaf(-(y - KV_ROUND), s, x);
+    // beyond half the scale, or at it with an odd code: one further (the bound is 0 for odd codes, the least number for even)
+    const float beyond = fmaf(2.f, fabsf(r), -s), bound = __uint_as_float((__float_as_uint(y) & 1u) ^ 1u);
+    return __float_as_uint(y + (beyond >= bound ? copysignf(1.f, r) : 0.f));
 }
-__device__ __forceinline__ int recode(int q, float s0, float s1, float ratio) {
-    const float f = (float)q * ratio;
-    float r = rintf(f);
-    if (fabsf(fabsf(f - r) - 0.5f) < 1e-4f || s0 < 1e-30f) r = (float)rint((double)q * (double)s0 / (double)s1);
-    return (int)r;
+// a code brought from scale s0 to s1: products of both sides of a border are compared in 64 bits, where they are exact
+__device__ __forceinline__ float kv_recode_border(float q, float c, float s0, float s1) {
+    const double num = (double)q * (double)s0, up = (c + 0.5) * (double)s1, down = (c - 0.5) * (double)s1;
+    const bool odd = (int)c & 1;
+    return num > up || (odd && num == up) ? c + 1.f : num < down || (odd && num == down) ? c - 1.f : c;
 }
-// the first ``keep`` of four codes in a word
+// scales below 1e-30 have reciprocals that do not fit: both sides are multiplied by 2^100 first, and what a scale rounded to
+// few bits leaves beyond 127 is cut
+#define KV_TINY 1e-30f
+#define KV_LIFT 1.2676506002282294e30f
+__device__ __forceinline__ float kv_lift(float x, float lifted) { return fminf(fmaxf(x * KV_LIFT, -127.f * lifted), 127.f * lifted); }
+// the first ``keep`` of four codes in a word, brought from scale s0 to s1
 __device__ __forceinline__ unsigned recode4(unsigned w, int keep, float s0, float s1, float ratio) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const unsigned q = (unsigned)recode((int8_t)(w >> (8 * i)), s0, s1, ratio) & 0xffu;
-        if (i < keep) w = (w & ~(0xffu << (8 * i))) | (q << (8 * i));
+        const float q = (float)(int8_t)(w >> (8 * i)), f = q * ratio;
+        float y = f + KV_ROUND;
+        if (fmaf(fabsf(f), KV_DOUBT, fabsf(f - (y - KV_ROUND))) > 0.5f) y = kv_recode_border(q, y - KV_ROUND, s0, s1) + KV_ROUND;
+        if (i < keep) w = (w & ~(0xffu << (8 * i))) | ((__float_as_uint(y) & 0xffu) << (8 * i));
     }
     return w;
 }
+// the lowest bytes of four words
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
 
-template <typename T, int W>
-__device__ __forceinline__ void append_run(const AppendSide<T>& a, bool values, const int32_t* __restrict__ slots, long slots_end,
-                                           int t, int n, int first, bool straight, int block, int head, int hk, int dk,
-                                           int block_size, bool pairs, int lane) {
+template <typename T, int W, bool VALUES>
+__device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t* __restrict__ slots, long slots_end, int t, int n,
+                                           int first, bool straight, int block, int head, int hk, int dk, int block_size, bool pairs,
+                                           int lane, int rank, int team, unsigned* tops) {
     constexpr int LR = W / 2, SUB = 64 / LR;                // lanes of a row, groups of 16 places side by side
     const int sub = lane / LR, c = 2 * (lane % LR);
     const T* x = a.x + (long)t * a.ld_row + (long)head * a.ld_head;
+    const int ld = (int)a.ld_row;
     const long at = (long)block * hk + head;
     int8_t* codes = a.codes + at * W * block_size;
     const int step = 16 * SUB, begin = first & ~15, end = first + n;
-    float v[16][2];
+    const float s0 = first == 0 ? 0.f : a.scale[at];
     struct alignas(2 * sizeof(T)) Pair { T e[2]; };
-    // the two columns of places base + 16 sub ...: all sixteen requests go out before the first is waited for, so rows and
-    // columns that are not there are read from ones that are, and dropped afterwards
+    Pair raw[16];                                           // two columns of 16 places, where all of the wave's are in the run
+    const auto full = [&](int base) { return pairs && base >= first && base + step <= end; };
     auto load = [&](int base) {
-        const int p0 = base + 16 * sub;
-        const int c0 = c < dk ? c : 0, c1 = c + 1 < dk ? c + 1 : 0;
-        Pair raw[16];
-        if (pairs && (dk & 1) == 0) {
+        unsigned off = ((base - first + 16 * sub) * ld + (c < dk ? c : 0)) * (unsigned)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) raw[i] = *(const Pair*)(x + (long)min(max(p0 + i - first, 0), n - 1) * a.ld_row + c0);
-        } else {
+        for (int i = 0; i < 16; ++i, off += ld * (unsigned)sizeof(T)) raw[i] = *(const Pair*)((const char*)x + off);
+        if (c >= dk) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const T* p = x + (long)min(max(p0 + i - first, 0), n - 1) * a.ld_row;
-                raw[i].e[0] = p[c0];
-                raw[i].e[1] = p[c1];
-            }
+            for (int i = 0; i < 16; ++i) raw[i].e[0] = raw[i].e[1] = from_f32<T>(0.f);
         }
+    };
+    // elsewhere (the ends of a run, single rows): four places at a time, each looked at by itself
+    auto load4 = [&](int p0, float (&f)[4][2]) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const bool in = p0 + i >= first && p0 + i < end;
-            v[i][0] = in && c < dk ? to_f32<T>(raw[i].e[0]) : 0.f;
-            v[i][1] = in && c + 1 < dk ? to_f32<T>(raw[i].e[1]) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+            const int r = p0 + i - first;
+            T e0 = from_f32<T>(0.f), e1 = e0;
+            if ((unsigned)r < (unsigned)n && c < dk) e0 = x[r * ld + c];
+            if ((unsigned)r < (unsigned)n && c + 1 < dk) e1 = x[r * ld + c + 1];
+            f[i][0] = to_f32<T>(e0);
+            f[i][1] = to_f32<T>(e1);
         }
     };
     unsigned top = 0;                                       // largest magnitude, as bits: NaN over infinity over numbers
     const auto mag = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
     if (straight) {
-        for (int base = begin; base < end; base += step) {
-            load(base);
+#pragma unroll 1
+        for (int base = begin + rank * step; base < end; base += team * step) {
+            if (full(base)) {
+                load(base);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = max(top, max(mag(v[i][0]), mag(v[i][1])));
+                for (int i = 0; i < 16; ++i) top = max(top, max(mag(to_f32<T>(raw[i].e[0])), mag(to_f32<T>(raw[i].e[1]))));
+            } else {
+#pragma unroll 1
+                for (int g = 0; g < 16; g += 4) {
+                    const int p0 = base + 16 * sub + g;
+                    if (!__any(p0 + 4 > first && p0 < end)) continue;
+                    float f[4][2];
+                    load4(p0, f);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = max(top, max(mag(f[i][0]), mag(f[i][1])));
+                }
+            }
         }
-    } else {
+    } else if (rank == 0) {
         for (int e = lane; e < n * dk; e += 64) {
             const int r = e / dk, s = slots[t + r];
             if (s >= 0 && s < slots_end) top = max(top, mag(to_f32<T>(x[(long)r * a.ld_row + (e - r * dk)])));
@@ -310,120 +338,178 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, bool values, 
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-    const float s0 = first == 0 ? 0.f : a.scale[at];
+    if (team > 1) {
+        if (lane == 0) tops[rank] = top;
+        __syncthreads();                                    // (every wave of the workgroup is here: teams go through runs together)
+        for (int i = 0; i < team; ++i) top = max(top, tops[i]);
+    }
+    top = __builtin_amdgcn_readfirstlane(top);
     // (as whole numbers, so that a scale that is not finite stays; it is kept as NaN)
     const unsigned bits = max(mag(s0), mag(__uint_as_float(top) / 127.f));
     const float s1 = __uint_as_float(bits < 0x7f800000u ? bits : 0x7fc00000u);
     if (s1 > s0 && first > 0) {
         const float ratio = s0 / s1;
-        const int words = values ? (first + 15) / 16 : first * W / 16, columns = values ? W : 1;
-        for (int e = lane; e < words * columns; e += 64) {
-            const int col = e / words, k = e - col * words;
-            uint4* p = (uint4*)(codes + (values ? col * block_size : 0) + 16 * k);
-            const int keep = values ? first - 16 * k : 16;
-            uint4 w = *p;
-            w.x = recode4(w.x, keep, s0, s1, ratio);
-            w.y = recode4(w.y, keep - 4, s0, s1, ratio);
-            w.z = recode4(w.z, keep - 8, s0, s1, ratio);
-            w.w = recode4(w.w, keep - 12, s0, s1, ratio);
-            *p = w;
+        // four codes at a time; those of the 16 places that ``first`` cuts belong to the wave that writes the others of them
+        const int whole = VALUES ? first / 16 * 4 : first * W / 4, columns = VALUES ? W : 1;
+#pragma unroll 1
+        for (int e = lane + 64 * rank; e < whole * columns; e += 64 * team) {
+            const int col = e / whole, k = e - col * whole;
+            unsigned* p = (unsigned*)(codes + col * block_size + 4 * k);
+            *p = recode4(*p, 4, s0, s1, ratio);
         }
-    }
-    const float inv = s1 > 0.f ? 1.f / s1 : 0.f;
-    if (straight) {
-        for (int base = begin; base < end; base += step) {
-            if (end - begin > step) load(base);             // (otherwise the registers hold the rows still)
-            const int p0 = base + 16 * sub;
-            if (values) {
-                if (p0 >= first && p0 + 16 <= end) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        unsigned w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[i] = 0;
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) w[i] |= ((unsigned)code_of(v[4 * i + r][k], s1, inv) & 0xffu) << (8 * r);
-                        }
-                        *(uint4*)(codes + (c + k) * block_size + p0) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (p0 + i >= first && p0 + i < end) {
-                            codes[c * block_size + p0 + i] = (int8_t)code_of(v[i][0], s1, inv);
-                            codes[(c + 1) * block_size + p0 + i] = (int8_t)code_of(v[i][1], s1, inv);
-                        }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (p0 + i >= first && p0 + i < end) {
-                        const unsigned two = ((unsigned)code_of(v[i][0], s1, inv) & 0xffu) | ((unsigned)code_of(v[i][1], s1, inv) & 0xffu) << 8;
-                        *(uint16_t*)(codes + (p0 + i) * W + c) = (uint16_t)two;
-                    }
+        if (VALUES && rank == 0 && (first & 15)) {
+#pragma unroll 1
+            for (int e = lane; e < 4 * W; e += 64) {
+                const int keep = (first & 15) - 4 * (e & 3);
+                unsigned* p = (unsigned*)(codes + (e >> 2) * block_size + 4 * whole + 4 * (e & 3));
+                if (keep > 0) *p = recode4(*p, keep, s0, s1, ratio);
             }
         }
-    } else {
+    }
+    const bool tiny = s1 > 0.f && s1 < KV_TINY;
+    // (a block of zeros has scale 0, and codes 0 beside any scale)
+    const float sd = tiny ? s1 * KV_LIFT : s1 == 0.f ? 3e38f : s1, inv = s1 > 0.f ? 1.f / sd : 0.f;
+    if (straight) {
+#pragma unroll 1
+        for (int base = begin + rank * step; base < end; base += team * step) {
+            if (full(base) && !tiny) {
+                if (end - begin > team * step) load(base);  // (otherwise the registers hold the rows still)
+                const int p0 = base + 16 * sub;
+                unsigned w[2][4];                           // codes of a column, four places to a word
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    unsigned q[4][2];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) q[i][k] = code_of(to_f32<T>(raw[4 * g + i].e[k]), sd, inv);
+                    if (VALUES) {
+                        w[0][g] = low_bytes(q[0][0], q[1][0], q[2][0], q[3][0]);
+                        w[1][g] = low_bytes(q[0][1], q[1][1], q[2][1], q[3][1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *(uint16_t*)(codes + (p0 + 4 * g + i) * W + c) = (uint16_t)__builtin_amdgcn_perm(q[i][1], q[i][0], 0x0c0c0400u);
+                    }
+                }
+                if (VALUES) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        *(uint4*)(codes + (c + k) * block_size + p0) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+                }
+            } else {
+#pragma unroll 1
+                for (int g = 0; g < 16; g += 4) {
+                    const int p0 = base + 16 * sub + g;
+                    if (!__any(p0 + 4 > first && p0 < end)) continue;
+                    float f[4][2];
+                    load4(p0, f);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (p0 + i < first || p0 + i >= end) continue;
+                        const unsigned q0 = code_of(tiny ? kv_lift(f[i][0], sd) : f[i][0], sd, inv),
+                                       q1 = code_of(tiny ? kv_lift(f[i][1], sd) : f[i][1], sd, inv);
+                        if (VALUES) {
+                            codes[c * block_size + p0 + i] = (int8_t)q0;
+                            codes[(c + 1) * block_size + p0 + i] = (int8_t)q1;
+                        } else *(uint16_t*)(codes + (p0 + i) * W + c) = (uint16_t)__builtin_amdgcn_perm(q1, q0, 0x0c0c0400u);
+                    }
+                }
+            }
+        }
+    } else if (rank == 0) {
         for (int r = 0; r < n; ++r) {                       // in the rows' order: of two rows for one place the later stays
             const int s = slots[t + r];
             if (s < 0 || s >= slots_end) continue;
             for (int col = lane; col < W; col += 64) {
-                const float f = col < dk ? to_f32<T>(x[(long)r * a.ld_row + col]) : 0.f;
-                codes[values ? col * block_size + s % block_size : (s % block_size) * W + col] = (int8_t)code_of(f, s1, inv);
+                float f = col < dk ? to_f32<T>(x[(long)r * a.ld_row + col]) : 0.f;
+                if (tiny) f = kv_lift(f, sd);
+                codes[VALUES ? col * block_size + s % block_size : (s % block_size) * W + col] = (int8_t)code_of(f, sd, inv);
             }
         }
     }
-    if (lane == 0) a.scale[at] = s1;
+    if (lane == 0 && rank == 0) a.scale[at] = s1;
 }
 
-template <typename T, int W>
-__global__ __launch_bounds__(256) void kv8_append_kernel(AppendSide<T> ks, AppendSide<T> vs, const int32_t* __restrict__ slots,
-                                                         int N, int rows_per_wg, int hk, int dk, int block_size, int k_pairs,
-                                                         int v_pairs, long slots_end) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, head = blockIdx.y;
-    const int t0 = blockIdx.x * rows_per_wg;
+#define KV_TEAM 4
+template <typename T, int W, bool VALUES>
+__device__ __forceinline__ void append_rows(const AppendSide<T>& a, const int32_t* __restrict__ slots, int N, int rows_per_wg, int hk,
+                                            int dk, int shift, bool pairs, long slots_end, unsigned (*tops)[KV_TEAM]) {
+    // (what is the same in all lanes of a wave is said to be, or the compiler keeps it per lane)
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, head = blockIdx.y;
+    const int t0 = blockIdx.x * rows_per_wg, block_size = 1 << shift;
     const auto good = [&](int s) { return s >= 0 && s < slots_end; };
+    // the slots of these rows and of the 64 behind them, in one trip to memory
+    const int sa = t0 + lane < N ? slots[t0 + lane] : -1, sb = t0 + 64 + lane < N ? slots[t0 + 64 + lane] : -1;
+    const int before = t0 > 0 ? slots[t0 - 1] : -1;
     // first rows of runs among the workgroup's rows; skipped rows do not end a run
     bool leads = false;
-    if (lane < rows_per_wg && t0 + lane < N) {
-        const int s = slots[t0 + lane];
-        if (good(s)) {
-            int p = t0 + lane - 1;
-            while (p >= 0 && !good(slots[p])) --p;
-            leads = p < 0 || slots[p] / block_size != s / block_size;
+    {
+        int p = __shfl_up(sa, 1, 64);
+        if (lane == 0) p = before;
+        if (lane < rows_per_wg && good(sa)) {
+            if (!good(p)) {
+                int i = t0 + lane - 2;
+                while (i >= 0 && !good(slots[i])) --i;
+                p = i >= 0 ? slots[i] : -1;
+            }
+            leads = !good(p) || p >> shift != sa >> shift;
         }
     }
-    unsigned long long found = __ballot(leads);
-    for (int job = 0; found; job += 2) {
-        const int t = t0 + __ffsll((long long)found) - 1;
+    unsigned long long found = __ballot(leads);             // (the same in every wave)
+    // few runs (chunks of prompts): teams of four waves; many (single tokens): a wave each
+    const int team = nw == KV_TEAM && __popcll(found) <= 2 ? KV_TEAM : 1, rank = team > 1 ? w : 0;
+    for (int run = 0; found; ++run) {
+        const int at = __ffsll((long long)found) - 1, t = t0 + at;
         found &= found - 1;
-        // both sides of a run go to neighbouring waves
-        for (int side = 0; side < 2; ++side) {
-            if ((job + side) % nw != w) continue;
-            const int s0 = slots[t], block = s0 / block_size;
-            int n = 0, first = block_size;                  // rows up to the run's last one, first place
-            bool straight = true, more = true;              // straight: no row skipped, places in order
+        if (team == 1 && run % nw != w) continue;
+        const int s0 = __builtin_amdgcn_readlane(sa, at), block = s0 >> shift;
+        // rows up to the run's last one, first place; straight: no row skipped, places in order (the usual run, and one that
+        // ends among the slots at hand)
+        const int ra = lane - at, rb = 64 - at + lane;
+        const unsigned long long stop_a = __ballot(ra >= 0 && sa != s0 + ra), stop_b = __ballot(sb != s0 + rb);
+        int n = min(stop_a ? __ffsll((long long)stop_a) - 1 - at : stop_b ? 64 - at + __ffsll((long long)stop_b) - 1 : 128 - at,
+                    block_size - (s0 & (block_size - 1)));
+        int first = s0 & (block_size - 1);
+        bool straight = t + n >= N;
+        if (!straight && at + n < 128) {                    // what stands behind decides: another block
+            const int behind = at + n < 64 ? __builtin_amdgcn_readlane(sa, at + n) : __builtin_amdgcn_readlane(sb, at + n - 64);
+            straight = good(behind) && behind >> shift != block;
+        }
+        if (!straight) {
+            n = 0;
+            first = block_size;
+            bool more = true, order = true;
             for (int r0 = 0; more; r0 += 64) {
                 const int r = r0 + lane, s = t + r < N ? slots[t + r] : -1;
-                const unsigned long long mine = __ballot(good(s) && s / block_size == block),
-                                         other = __ballot(t + r >= N || (good(s) && s / block_size != block));
-                const unsigned long long in = other ? mine & ((other & -other) - 1) : mine;
+                const unsigned long long same = __ballot(good(s) && s >> shift == block),
+                                         other = __ballot(t + r >= N || (good(s) && s >> shift != block));
+                const unsigned long long in = other ? same & ((other & -other) - 1) : same;
                 more = !other;
                 if (in) {
                     const int last = 63 - __clzll((long long)in);
-                    straight = straight && n == r0 && __ballot(lane <= last && s != s0 + r) == 0;
+                    order = order && n == r0 && __ballot(lane <= last && s != s0 + r) == 0;
                     n = r0 + last + 1;
-                    int p = (in >> lane) & 1 ? s % block_size : block_size;
+                    int p = (in >> lane) & 1 ? s & (block_size - 1) : block_size;
 #pragma unroll
                     for (int o = 32; o > 0; o >>= 1) p = min(p, __shfl_xor(p, o, 64));
-                    first = min(first, p);
+                    first = min(first, __builtin_amdgcn_readfirstlane(p));
                 }
             }
-            if (side) append_run<T, W>(vs, true, slots, slots_end, t, n, first, straight, block, head, hk, dk, block_size, v_pairs, lane);
-            else append_run<T, W>(ks, false, slots, slots_end, t, n, first, straight, block, head, hk, dk, block_size, k_pairs, lane);
+            straight = order;
         }
+        append_run<T, W, VALUES>(a, slots, slots_end, t, n, first, straight, block, head, hk, dk, block_size, pairs, lane, rank, team,
+                                 tops[run & 1]);
     }
+}
+
+template <typename T, int W>
+__global__ __launch_bounds__(64 * KV_TEAM) void kv8_append_kernel(AppendSide<T> ks, AppendSide<T> vs, const int32_t* __restrict__ slots,
+                                                                 int N, int rows_per_wg, int hk, int dk, int shift, int k_pairs,
+                                                                 int v_pairs, long slots_end) {
+    __shared__ unsigned tops[2][KV_TEAM];
+    if (blockIdx.z) append_rows<T, W, true>(vs, slots, N, rows_per_wg, hk, dk, shift, v_pairs, slots_end, tops);
+    else append_rows<T, W, false>(ks, slots, N, rows_per_wg, hk, dk, shift, k_pairs, slots_end, tops);
 }
 
 static int kv8_check(const char* name, int num_blocks, int hk, int block_size, int dk, int width) {
@@ -452,16 +538,19 @@ extern "C" int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_
     float *k_scale = d->k_scale, *v_scale = d->v_scale;
     ATHENA_REQUIRE(k && v && slots && k_codes && v_codes && k_scale && v_scale, ATHENA_E_SHAPE, "athena_kv8_append: null operand");
     ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN, "athena_kv8_append: codes must lie on 16 bytes");
-    const int per = (long)N * hk <= 4096 ? 1 : 16;
-    const dim3 grid((N + per - 1) / per, hk), block(per == 1 ? 128 : 256);
+    ATHENA_REQUIRE(ldk >= 0 && ldv >= 0 && ldk < (1 << 22) && ldv < (1 << 22), ATHENA_E_SHAPE,
+                   "athena_kv8_append: rows %ld / %ld elements apart (2^22 at most)", ldk, ldv);
+    const int per = (long)N * hk <= 4096 ? 1 : 64;
+    const dim3 grid((N + per - 1) / per, hk, 2), block(per == 1 ? 64 : 64 * KV_TEAM);
     const long end = (long)num_blocks * block_size;
+    const int shift = __builtin_ctz(block_size);
     const size_t two = d->dtype == ATHENA_BF16 ? 4 : 8;        // two elements in one load where rows and heads begin on them
-    const int kp = (uintptr_t)k % two == 0 && ldk % 2 == 0 && ldk_head % 2 == 0;
-    const int vp = (uintptr_t)v % two == 0 && ldv % 2 == 0 && ldv_head % 2 == 0;
+    const int kp = (uintptr_t)k % two == 0 && ldk % 2 == 0 && ldk_head % 2 == 0 && dk % 2 == 0;
+    const int vp = (uintptr_t)v % two == 0 && ldv % 2 == 0 && ldv_head % 2 == 0 && dk % 2 == 0;
 #define KV_APPEND(T, W)                                                                                                     \
     do {                                                                                                                    \
         AppendSide<T> ks = {(const T*)k, ldk, ldk_head, k_codes, k_scale}, vs = {(const T*)v, ldv, ldv_head, v_codes, v_scale}; \
-        ATHENA_LAUNCH((kv8_append_kernel<T, W>), grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, block_size, \
+        ATHENA_LAUNCH((kv8_append_kernel<T, W>), grid, block, 0, (hipStream_t)stream, ks, vs, slots, N, per, hk, dk, shift,      \
                       kp, vp, end);                                                                                         \
     } while (0)
 #define KV_APPEND_W(T)                     \
