@@ -1,8 +1,7 @@
 // Attention over the 8-bit paged cache on the matrix cores (fp16 operands, fp32 softmax and accumulation).
 //
-// A wave owns RT tiles of 16 query rows (row = new token x query head of one kv head) and walks its share of the
-// sequence in tiles of 64 tokens; the four waves of a workgroup take every fourth tile and meet once, at the end.
-// Nothing is staged: codes go from memory into registers, are widened there, and are the matrix operands.
+// A wave owns RT tiles of 16 query rows (row = new token x query head of one kv head) and walks tokens in tiles of 64.
+// Sequences with few rows (single new tokens) and with many (chunks of prompts) have a kernel each, see there.
 //   S^T = K Q^T   A = 16 keys x 32 columns, B = 32 columns x 16 queries.  Which keys make a tile's rows is free:
 //                 tile t (of 4) takes keys 16 (m >> 2) + 4 t + (m & 3), so that lane group g = lane >> 4 ends up
 //                 with the 16 consecutive keys 16 g .. 16 g + 15 of its query (lane & 15).  The order of the
@@ -37,12 +36,13 @@ struct KvAttn {
     long ldo, ldo_head;
     float* lse;             // [N][h] or null
     float *part, *part_lse; // [splits][N][h][dk], [splits][N][h]: used where the key axis is split
-    int table_width, num_blocks, B, N, h, hk, dk, block_size, causal, splits, row_tiles, q_wide, out_wide;
+    int table_width, num_blocks, B, N, h, hk, dk, block_size, block_shift, causal, splits, row_tiles, few, q_wide, out_wide;     // few: rows up to which a sequence's key axis is divided
     float scale;
 };
 
 #define KV_KEYS 64          // tokens of a tile
 #define KV_MIN_TILES 16     // tiles of a split at least
+#define KV_FEW 64           // rows of a (sequence, kv head) up to which the key axis is what is divided
 
 // eight codes as fp16: bytes b of code + 128 become 1024 + b (0x6400 | b), less 1152
 __device__ __forceinline__ f16x8_t kv_widen(unsigned lo, unsigned hi) {
@@ -85,9 +85,184 @@ template <int W> __device__ __forceinline__ int kv_column(int f, int g) {
     return W == 32 ? 8 * g : 64 * (f >> 1) + 16 * g + 8 * (f & 1);
 }
 
+// Queries of RT tiles of 16 rows from row ``row0`` of a (sequence, kv head), scaled by a power of two to [1, 2), as operands;
+// what the power and the softmax's scale come to (``qs``, for exponents of two); how many tokens each row sees.
+template <typename T, int W, int RT> struct KvQueries {
+    static constexpr bool TWO = sizeof(T) == 4;             // fp32: queries and probabilities in two fp16 numbers
+    static constexpr int F = W / 32;
+    f16x8_t q[RT][F], ql[TWO ? RT : 1][TWO ? F : 1];
+    float qs[RT];
+    int limit[RT], least, most;                             // of a lane's rows; the fewest and the most of the wave's
+    __device__ __forceinline__ void load(const KvAttn& a, int kvh, int G, int lo, int n, int len, long row0, int qc, int g) {
+        least = 0x7fffffff;
+        most = 0;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const long row = row0 + 16 * r + qc;
+            const bool in = row < (long)n * G;
+            const int token = in ? (int)(row / G) : 0, head = kvh * G + (in ? (int)(row % G) : 0);
+            limit[r] = !in ? 0 : a.causal ? min(max(len - n + token + 1, 0), len) : len;
+            const T* p = (const T*)a.q + (long)(lo + token) * a.ldq + (long)head * a.ldq_head;
+            float v[F][8], top = 0.f;
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                const int c = kv_column<W>(f, g);
+                if (in && a.q_wide && c < a.dk) {
+                    struct alignas(16) Eight { T e[8]; };
+                    const Eight x = *(const Eight*)(p + c);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[f][i] = to_f32<T>(x.e[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[f][i] = in && c + i < a.dk ? to_f32<T>(p[c + i]) : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[f][i]));
+            }
+            const unsigned e = min(max(__float_as_uint(rows4_max(top)) >> 23, 1u), 253u);
+            const float down = __uint_as_float((254u - e) << 23);
+            qs[r] = a.scale * 1.4426950408889634f * __uint_as_float(e << 23);
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = v[f][i] * down;
+                    q[r][f][i] = (f16_t)x;
+                    if (TWO) ql[r][f][i] = (f16_t)(x - (float)q[r][f][i]);
+                }
+            least = min(least, in ? limit[r] : 0x7fffffff);
+            most = max(most, limit[r]);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            least = min(least, __shfl_xor(least, o, 64));
+            most = max(most, __shfl_xor(most, o, 64));
+        }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
+    }
+    __device__ __forceinline__ void score(f32x4_t& s, f16x8_t k, int r, int f) const {
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[r][f], s, 0, 0, 0);
+        if (TWO) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[r][f], s, 0, 0, 0);
+    }
+};
+
+// One tile of 64 keys of one tile of 16 rows: the running maxima and sum, and probability times value scale as operands.
+// ``ksq`` (not negative) brings scores to exponents of two, ``vs`` is the lane's value scale, ``vl`` its logarithm to base 2.
+template <int W, bool TWO> struct KvSoftmax {
+    f32x4_t o[W / 16];
+    float m, l, m2;
+    __device__ __forceinline__ void begin() {
+        m = m2 = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < W / 16; ++d) o[d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void tile(f32x4_t (&s)[4], float ksq, float vs, float vl, bool whole, int seen, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][e] = 4 * i + e < seen ? s[i][e] : -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
+        // (a scale of 0 beside a score of -inf, which is "hidden": still hidden)
+        top = top == -INFINITY ? top : top * ksq;
+        const float mn = fmaxf(m, rows4_max(top)), mn2 = fmaxf(m2, rows4_max(top + vl));
+        const float base = mn == -INFINITY ? 0.f : mn, base2 = mn2 == -INFINITY ? 0.f : mn2;
+        if (__any(mn > m || mn2 > m2)) {
+            l *= __builtin_amdgcn_exp2f(m - base);
+            const float down = __builtin_amdgcn_exp2f(m2 - base2);
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d][e] *= down;
+            m = mn;
+            m2 = mn2;
+        }
+        // Probability times value scale in one exponential, and the sum of the lane's sixteen divided by the scale again.
+        // Where the scale is far below the largest product so far (or 0, or not finite) that division would lose the
+        // probabilities: they are then worked out by themselves.
+        const float shift = vl + base - base2;
+        if (whole && !__any(!(shift > -40.f))) {
+            const float at = vl - base2;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, at));
+                    sum += s[i][e];
+                }
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+        } else {                                            // scales that are 0 or not finite must not reach hidden keys
+            const float vf = fminf(vs * __builtin_amdgcn_exp2f(base - base2), 3.4e38f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool hidden = s[i][e] == -INFINITY;
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, -base));
+                    l += hidden ? 0.f : x;
+                    s[i][e] = hidden ? 0.f : x * vf;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f16_t h = (f16_t)s[i][e];
+                p[i >> 1][4 * (i & 1) + e] = h;
+                if (TWO) pl[i >> 1][4 * (i & 1) + e] = (f16_t)(s[i][e] - (float)h);
+            }
+    }
+    __device__ __forceinline__ void add(int d, f16x8_t v, const f16x8_t& p, const f16x8_t& pl) {
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o[d], 0, 0, 0);
+        if (TWO) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[d], 0, 0, 0);
+    }
+};
+
+// rows of a sequence that the kernel of few rows takes; the others go to the kernel of many
+__device__ __forceinline__ bool kv_few(const KvAttn& a, int n) { return (long)n * (a.h / a.hk) <= a.few; }
+
+// four columns of a row's result: sum ``y`` over the sum of exponentials ``l`` relative to 2^base; with a split key axis to that
+// split's part of the workspace.
+template <typename T>
+__device__ __forceinline__ void kv_finish(const KvAttn& a, long token, long head, int c, float base, float l, f32x4_t y, int split) {
+    // nothing seen: zeros; NaN stays
+    const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;
+    const float lse = l > 0.f ? base + __builtin_amdgcn_logf(l) : l != l ? l : -INFINITY;
+    if (a.splits > 1) {
+        const long at = ((long)split * a.N + token) * a.h + head;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < a.dk) a.part[at * a.dk + c + j] = y[j] * inv;
+        if (c == 0) a.part_lse[at] = lse;
+        return;
+    }
+    T* out = (T*)a.out + token * a.ldo + head * a.ldo_head + c;
+    if (a.out_wide && c + 4 <= a.dk) {
+        struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) four.e[j] = from_f32<T>(y[j] * inv);
+        *(Four*)out = four;
+    } else {
+        for (int j = 0; j < 4; ++j)
+            if (c + j < a.dk) out[j] = from_f32<T>(y[j] * inv);
+    }
+    if (a.lse && c == 0) a.lse[token * a.h + head] = lse * 0.6931471805599453f;
+}
+
+// ---------------------------------------------------------------- few rows: bound by the cache's way in
+// The four waves of a workgroup take every fourth tile of its share of the keys and meet once, at the end; a lane's codes go
+// from memory straight into operands.
 template <typename T, int W, int RT>
 __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
-    constexpr bool TWO = sizeof(T) == 4;    // fp32: queries and probabilities in two fp16 numbers
+    constexpr bool TWO = sizeof(T) == 4;
     constexpr int F = W / 32, D = W / 16, ROWS = 16 * RT;
     __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_m2[4][ROWS];
     __shared__ float s_o[4][ROWS][W + 4];
@@ -102,69 +277,18 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
     const int n = hi - lo;
     const int len = (int)min((long long)max(a.lens[b], 0), (long long)a.table_width * a.block_size);
     const int32_t* table = a.tables + (long)b * a.ld_tables;
+    if (!kv_few(a, n)) return;
 
     for (long tile0 = (long)(part / a.splits) * ROWS; tile0 < (long)n * G; tile0 += (long)a.row_tiles * ROWS) {
-        // ---- this wave's queries
-        f16x8_t qf[RT][F], ql[TWO ? RT : 1][TWO ? F : 1];
-        float qs[RT];
-        int limit[RT], least = 0x7fffffff, most = 0;        // tokens a row sees; the fewest and the most of the tile
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const long row = tile0 + 16 * r + qc;
-            const bool in = row < (long)n * G;
-            const int token = in ? (int)(row / G) : 0, head = kvh * G + (in ? (int)(row % G) : 0);
-            limit[r] = !in ? 0 : a.causal ? min(max(len - n + token + 1, 0), len) : len;
-            const T* q = (const T*)a.q + (long)(lo + token) * a.ldq + (long)head * a.ldq_head;
-            float v[F][8], top = 0.f;
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
-                const int c = kv_column<W>(f, g);
-                if (in && a.q_wide && c < a.dk) {
-                    struct alignas(16) Eight { T e[8]; };
-                    const Eight x = *(const Eight*)(q + c);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[f][i] = to_f32<T>(x.e[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[f][i] = in && c + i < a.dk ? to_f32<T>(q[c + i]) : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[f][i]));
-            }
-            const unsigned e = min(max(__float_as_uint(rows4_max(top)) >> 23, 1u), 253u);
-            const float down = __uint_as_float((254u - e) << 23);
-            qs[r] = a.scale * 1.4426950408889634f * __uint_as_float(e << 23);
-#pragma unroll
-            for (int f = 0; f < F; ++f)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = v[f][i] * down;
-                    qf[r][f][i] = (f16_t)x;
-                    if (TWO) ql[r][f][i] = (f16_t)(x - (float)qf[r][f][i]);
-                }
-            least = min(least, limit[r]);
-            most = max(most, limit[r]);
-        }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            least = min(least, __shfl_xor(least, o, 64));
-            most = max(most, __shfl_xor(most, o, 64));
-        }
-        least = __builtin_amdgcn_readfirstlane(least);
-        most = __builtin_amdgcn_readfirstlane(most);
+        KvQueries<T, W, RT> q;
+        q.load(a, kvh, G, lo, n, len, tile0, qc, g);
         // ---- this workgroup's tiles of keys
-        const int tiles = (most + KV_KEYS - 1) / KV_KEYS;
+        const int tiles = (q.most + KV_KEYS - 1) / KV_KEYS;
         const int per = a.splits > 1 ? max((tiles + a.splits - 1) / a.splits, KV_MIN_TILES) : tiles;
         const int t_end = min((split + 1) * per, tiles);
-        f32x4_t o[RT][D];
-        float m[RT], l[RT], m2[RT];
+        KvSoftmax<W, TWO> x[RT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            m[r] = m2[r] = -INFINITY;
-            l[r] = 0.f;
-#pragma unroll
-            for (int d = 0; d < D; ++d) o[r][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-        }
+        for (int r = 0; r < RT; ++r) x[r].begin();
         KvKeys<W> k;
         uint4 v[D];
         float ks, vs;
@@ -173,21 +297,21 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
         const int kc = 16 * (qc >> 2), vc = 16 * g;         // where in a tile they begin
         auto find = [&](int t) {
             const int jk = t * KV_KEYS + kc, jv = t * KV_KEYS + vc;
-            kb = t < t_end && jk < most ? table[jk / a.block_size] : -1;
-            vb = t < t_end && jv < most ? table[jv / a.block_size] : -1;
+            kb = t < t_end && jk < q.most ? table[jk >> a.block_shift] : -1;
+            vb = t < t_end && jv < q.most ? table[jv >> a.block_shift] : -1;
         };
         auto load_keys = [&](int t) {
-            const int at = (t * KV_KEYS + kc) % a.block_size + (qc & 3);
+            const int at = ((t * KV_KEYS + kc) & (a.block_size - 1)) + (qc & 3);
             const int block = (unsigned)kb < (unsigned)a.num_blocks ? kb : 0;
-            k.load(a.k_codes + (((long)block * a.hk + kvh) * a.block_size + at) * W + (W == 32 ? 8 : 16) * g);
+            k.load(a.k_codes + ((((long)block * a.hk + kvh) << a.block_shift) + at) * W + (W == 32 ? 8 : 16) * g);
             ok = (unsigned)vb < (unsigned)a.num_blocks;
             const long scale_at = (long)(ok ? vb : 0) * a.hk + kvh;
             ks = a.k_scale[scale_at];
             vs = a.v_scale[scale_at];
         };
         auto load_values = [&](int t, int block) {
-            const int at = (t * KV_KEYS + vc) % a.block_size;
-            const int8_t* p = a.v_codes + (((long)((unsigned)block < (unsigned)a.num_blocks ? block : 0) * a.hk + kvh) * W + qc) * a.block_size + at;
+            const int at = (t * KV_KEYS + vc) & (a.block_size - 1);
+            const int8_t* p = a.v_codes + ((((long)((unsigned)block < (unsigned)a.num_blocks ? block : 0) * a.hk + kvh) * W + qc) << a.block_shift) + at;
 #pragma unroll
             for (int d = 0; d < D; ++d) v[d] = *(const uint4*)(p + d * 16 * a.block_size);
         };
@@ -202,7 +326,6 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
             const bool next = t + 4 < t_end;
             const float ks_now = ks, vs_now = vs;
             const bool ok_now = ok;
-            // ---- scores
             f32x4_t s[RT][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -212,92 +335,25 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
                 for (int f = 0; f < F; ++f) {
                     const f16x8_t kf = k.frag(i, f);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[r][f], s[r][i], 0, 0, 0);
-                        if (TWO) s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[r][f], s[r][i], 0, 0, 0);
-                    }
+                    for (int r = 0; r < RT; ++r) q.score(s[r][i], kf, r, f);
                 }
             }
             const int block_next = vb;
             if (next) load_keys(t + 4);
-            const bool whole = !__any(!ok_now) && (t + 1) * KV_KEYS <= least;
+            const bool whole = !__any(!ok_now) && (t + 1) * KV_KEYS <= q.least;
             const int j0 = t * KV_KEYS + vc;
             const float vl = __builtin_amdgcn_logf(fabsf(vs_now));          // log2
-            // ---- softmax
-            f16x8_t p[RT][2], pl[TWO ? RT : 1][2];
+            f16x8_t p[RT][2], pl[RT][2];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const float ksq = ks_now * qs[r];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[r][i][e] *= ksq;
-                if (!whole) {
-                    const int seen = ok_now ? limit[r] - j0 : 0;            // this lane's keys below it are visible
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[r][i][e] = 4 * i + e < seen ? s[r][i][e] : -INFINITY;
-                }
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, s[r][i][e]);
-                const float mn = fmaxf(m[r], rows4_max(top)), mn2 = fmaxf(m2[r], rows4_max(top + vl));
-                const float base = mn == -INFINITY ? 0.f : mn, base2 = mn2 == -INFINITY ? 0.f : mn2;
-                if (__any(mn > m[r] || mn2 > m2[r])) {
-                    l[r] *= __builtin_amdgcn_exp2f(m[r] - base);
-                    const float down = __builtin_amdgcn_exp2f(m2[r] - base2);
-#pragma unroll
-                    for (int d = 0; d < D; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[r][d][e] *= down;
-                    m[r] = mn;
-                    m2[r] = mn2;
-                }
-                const float vf = fminf(vs_now * __builtin_amdgcn_exp2f(base - base2), 3.4e38f);
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[r][i][e] = __builtin_amdgcn_exp2f(s[r][i][e] - base);
-                        sum += s[r][i][e];
-                    }
-                if (whole) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[r][i][e] *= vf;
-                } else {                                    // a scale that is not finite must not reach hidden keys
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[r][i][e] = s[r][i][e] == 0.f ? 0.f : s[r][i][e] * vf;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const f16_t h = (f16_t)s[r][i][e];
-                        p[r][i >> 1][4 * (i & 1) + e] = h;
-                        if (TWO) pl[r][i >> 1][4 * (i & 1) + e] = (f16_t)(s[r][i][e] - (float)h);
-                    }
-                l[r] += sum;
-            }
-            // ---- values
+            for (int r = 0; r < RT; ++r)
+                x[r].tile(s[r], ks_now * q.qs[r], vs_now, vl, whole, ok_now ? q.limit[r] - j0 : 0, p[r], pl[r]);
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 const f16x8_t v0 = kv_widen(v[d].x, v[d].y), v1 = kv_widen(v[d].z, v[d].w);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[r][0], o[r][d], 0, 0, 0);
-                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[r][1], o[r][d], 0, 0, 0);
-                    if (TWO) {
-                        o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[r][0], o[r][d], 0, 0, 0);
-                        o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[r][1], o[r][d], 0, 0, 0);
-                    }
+                    x[r].add(d, v0, p[r][0], pl[r][0]);
+                    x[r].add(d, v1, p[r][1], pl[r][1]);
                 }
             }
             if (next) {
@@ -309,14 +365,14 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
         __syncthreads();                                    // (the rows before are done with the shared memory)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            l[r] = rows4_sum(l[r]);
+            const float l = rows4_sum(x[r].l);
             if (g == 0) {
-                s_m[w][16 * r + qc] = m[r];
-                s_l[w][16 * r + qc] = l[r];
-                s_m2[w][16 * r + qc] = m2[r];
+                s_m[w][16 * r + qc] = x[r].m;
+                s_l[w][16 * r + qc] = l;
+                s_m2[w][16 * r + qc] = x[r].m2;
             }
 #pragma unroll
-            for (int d = 0; d < D; ++d) *(f32x4_t*)&s_o[w][16 * r + qc][16 * d + 4 * g] = o[r][d];
+            for (int d = 0; d < D; ++d) *(f32x4_t*)&s_o[w][16 * r + qc][16 * d + 4 * g] = x[r].o[d];
         }
         __syncthreads();
         constexpr int CG = W / 4;                           // groups of four columns
@@ -329,39 +385,166 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
             for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s_m[i][rr]);
             const float base = mt == -INFINITY ? 0.f : mt;
             float lt = 0.f;
-            f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+            f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 lt += s_l[i][rr] * __builtin_amdgcn_exp2f(s_m[i][rr] - base);
                 const float up = s_m2[i][rr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m2[i][rr] - base);
-                const f32x4_t y = *(const f32x4_t*)&s_o[i][rr][c];
+                const f32x4_t z = *(const f32x4_t*)&s_o[i][rr][c];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] += y[j] * up;
+                for (int j = 0; j < 4; ++j) y[j] += z[j] * up;
             }
-            // nothing seen: zeros; NaN stays
-            const float inv = lt > 0.f ? 1.f / lt : lt != lt ? lt : 0.f;
-            const float lse = lt > 0.f ? base + __builtin_amdgcn_logf(lt) : lt != lt ? lt : -INFINITY;
-            const long token = lo + row / G, head = kvh * G + row % G;
-            if (a.splits > 1) {
-                const long at = ((long)split * a.N + token) * a.h + head;
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < a.dk) a.part[at * a.dk + c + j] = x[j] * inv;
-                if (c == 0) a.part_lse[at] = lse;
-            } else {
-                T* out = (T*)a.out + token * a.ldo + head * a.ldo_head + c;
-                if (a.out_wide && c + 4 <= a.dk) {
-                    struct alignas(4 * sizeof(T)) Four { T e[4]; } four;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) four.e[j] = from_f32<T>(x[j] * inv);
-                    *(Four*)out = four;
-                } else {
-                    for (int j = 0; j < 4; ++j)
-                        if (c + j < a.dk) out[j] = from_f32<T>(x[j] * inv);
-                }
-                if (a.lse && c == 0) a.lse[token * a.h + head] = lse * 0.6931471805599453f;
-            }
+            kv_finish<T>(a, lo + row / G, kvh * G + row % G, c, base, lt, y, split);
         }
         __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- many rows: bound by the vector and matrix units
+// A wave owns 16 RT rows, the NW waves of a workgroup walk its share of the keys together: a tile is loaded once (each thread a few
+// 16-byte pieces), widened once and left in LDS as fp16, double-buffered, one barrier a tile.  Widening took more
+// vector instructions than the softmax when every wave did it for itself.
+// LDS images in 16-byte chunks (8 numbers), placed so that the 8 lanes that read side by side hit 8 different groups of
+// banks: keys [64][W], chunk ^ swz(key); values [W][64], chunk ^ (column & 7).
+template <int W> __device__ __forceinline__ int kv_swz(int key) {
+    return W == 32 ? (key >> 4) & 3 : (key & 3) | ((key >> 4) & 1) << 2;
+}
+
+template <typename T, int W, int RT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv8_attention_rows_kernel(KvAttn a) {
+    constexpr bool TWO = sizeof(T) == 4;
+    constexpr int F = W / 32, D = W / 16, NT = 64 * NW, ROWS = 16 * NW * RT, NC = W / 8, PIECES = 4 * W, NP = (PIECES + NT - 1) / NT;
+    __shared__ __attribute__((aligned(16))) f16_t s_k[2][64 * W], s_v[2][64 * W];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, qc = lane & 15;
+    const int inner = a.row_tiles * a.splits, unit = blockIdx.x / 8, part = unit % inner;
+    const int pair = unit / inner * 8 + blockIdx.x % 8;
+    if (pair >= a.B * a.hk) return;
+    const int b = pair / a.hk, kvh = pair % a.hk, split = part % a.splits, G = a.h / a.hk;
+    const int lo = min(max(a.cu_rows ? a.cu_rows[b] : b, 0), a.N), hi = min(max(a.cu_rows ? a.cu_rows[b + 1] : b + 1, lo), a.N);
+    const int n = hi - lo;
+    const int len = (int)min((long long)max(a.lens[b], 0), (long long)a.table_width * a.block_size);
+    const int32_t* table = a.tables + (long)b * a.ld_tables;
+    if (kv_few(a, n)) return;
+    // where this lane's fragments lie in the images: keys 16 (qc >> 2) + (qc & 3) + 4 i, columns qc + 16 d
+    const int key0 = 16 * (qc >> 2) + (qc & 3), z = kv_swz<W>(key0);
+    const int at_k0 = key0 * W + (((W == 32 ? g : 2 * g) ^ z) * 8), at_k1 = key0 * W + (((2 * g + 1) ^ z) * 8);
+    const int at_v0 = qc * 64 + (((2 * g) ^ (qc & 7)) * 8), at_v1 = qc * 64 + (((2 * g + 1) ^ (qc & 7)) * 8);
+    const long row_tiles = ((long)n * G + ROWS - 1) / ROWS;
+    for (long i = part / a.splits; i < row_tiles; i += a.row_tiles) {
+        const long tile0 = (row_tiles - 1 - i) * ROWS, row0 = tile0 + w * 16 * RT;     // causal: the longest rows begin first
+        KvQueries<T, W, RT> q;
+        q.load(a, kvh, G, lo, n, len, row0, qc, g);
+        const int last = (int)min(tile0 + ROWS, (long)n * G) - 1, most = a.causal ? min(max(len - n + last / G + 1, 0), len) : len;
+        const int all = (most + KV_KEYS - 1) / KV_KEYS, per = a.splits > 1 ? max((all + a.splits - 1) / a.splits, KV_MIN_TILES) : all;
+        const int begin = min(split * per, all), tiles = min(begin + per, all);         // this workgroup's tiles of keys
+        KvSoftmax<W, TWO> x[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) x[r].begin();
+        // ---- staging: this thread's pieces of 16 codes
+        uint4 kr[NP], vr[NP];
+        int kb[NP], vb, sb;                                 // blocks of the tile to load next: keys, values, scales
+        float ks = 0.f, vs = 0.f;
+        bool ok = false;
+        const auto lookup = [&](int t, int j) { return t < tiles && t * KV_KEYS + j < most ? table[(t * KV_KEYS + j) >> a.block_shift] : -1; };
+        const auto inside = [&](int block) { return (unsigned)block < (unsigned)a.num_blocks ? block : 0; };
+        auto find = [&](int t) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) kb[p] = lookup(t, (tid + NT * p) / (W / 16) & 63);
+            vb = lookup(t, 16 * (tid & 3));
+            sb = lookup(t, 16 * g);
+        };
+        auto load = [&](int t) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int e = tid + NT * p, key = e / (W / 16), d = e >> 2;
+                if (PIECES < NT && e >= PIECES) continue;
+                kr[p] = *(const uint4*)(a.k_codes + ((((long)inside(kb[p]) * a.hk + kvh) << a.block_shift) + ((t * KV_KEYS + key) & (a.block_size - 1))) * W + 16 * (e % (W / 16)));
+                vr[p] = *(const uint4*)(a.v_codes + ((((long)inside(vb) * a.hk + kvh) * W + d) << a.block_shift) + ((t * KV_KEYS + 16 * (e & 3)) & (a.block_size - 1)));
+            }
+        };
+        auto load_scales = [&] {
+            ok = (unsigned)sb < (unsigned)a.num_blocks;
+            const long at = (long)(ok ? sb : 0) * a.hk + kvh;
+            ks = a.k_scale[at];
+            vs = a.v_scale[at];
+        };
+        auto stage = [&](int buf) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int e = tid + NT * p, key = e / (W / 16), c = 2 * (e % (W / 16)), d = e >> 2, cv = 2 * (e & 3);
+                if (PIECES < NT && e >= PIECES) continue;
+                *(f16x8_t*)&s_k[buf][(key * NC + (c ^ kv_swz<W>(key))) * 8] = kv_widen(kr[p].x, kr[p].y);
+                *(f16x8_t*)&s_k[buf][(key * NC + ((c + 1) ^ kv_swz<W>(key))) * 8] = kv_widen(kr[p].z, kr[p].w);
+                *(f16x8_t*)&s_v[buf][(d * 8 + (cv ^ (d & 7))) * 8] = kv_widen(vr[p].x, vr[p].y);
+                *(f16x8_t*)&s_v[buf][(d * 8 + ((cv + 1) ^ (d & 7))) * 8] = kv_widen(vr[p].z, vr[p].w);
+            }
+        };
+        __syncthreads();                                    // (the rows before are done with the shared memory)
+        if (begin < tiles) {
+            find(begin);
+            load(begin);
+            load_scales();
+            find(begin + 1);
+            stage(begin & 1);
+        }
+        __syncthreads();
+        for (int t = begin; t < tiles; ++t) {
+            const float ks_now = ks, vs_now = vs;
+            const bool ok_now = ok, next = t + 1 < tiles;
+            if (next) {
+                load(t + 1);
+                load_scales();
+                find(t + 2);
+            }
+            if (t * KV_KEYS < q.most) {                     // (a causal wave is done before the workgroup's last rows are)
+                // (the XORs depend on the lane alone: everything else is a constant distance from these four places)
+                const f16_t *sk0 = s_k[t & 1] + at_k0, *sk1 = s_k[t & 1] + at_k1, *sv0 = s_v[t & 1] + at_v0, *sv1 = s_v[t & 1] + at_v1;
+                f32x4_t s[RT][4];
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) s[r][i4] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int f = 0; f < F; ++f) {
+                        const f16x8_t kf = *(const f16x8_t*)((f & 1 ? sk1 : sk0) + i4 * 4 * W + (f >> 1) * 64);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) q.score(s[r][i4], kf, r, f);
+                    }
+                }
+                const bool whole = !__any(!ok_now) && (t + 1) * KV_KEYS <= q.least;
+                const int j0 = t * KV_KEYS + 16 * g;
+                const float vl = __builtin_amdgcn_logf(fabsf(vs_now));      // log2
+                f16x8_t p[RT][2], pl[RT][2];
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    x[r].tile(s[r], ks_now * q.qs[r], vs_now, vl, whole, ok_now ? q.limit[r] - j0 : 0, p[r], pl[r]);
+#pragma unroll
+                for (int d = 0; d < D; ++d) {
+                    const f16x8_t v0 = *(const f16x8_t*)(sv0 + d * 16 * 64), v1 = *(const f16x8_t*)(sv1 + d * 16 * 64);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        x[r].add(d, v0, p[r][0], pl[r][0]);
+                        x[r].add(d, v1, p[r][1], pl[r][1]);
+                    }
+                }
+            }
+            if (next) stage((t + 1) & 1);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const long row = row0 + 16 * r + qc;
+            const float l = rows4_sum(x[r].l), base = x[r].m == -INFINITY ? 0.f : x[r].m;
+            const float up = x[r].m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[r].m2 - base);
+            if (row >= (long)n * G) continue;
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                f32x4_t y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = x[r].o[d][j] * up;
+                kv_finish<T>(a, lo + row / G, kvh * G + row % G, 16 * d + 4 * g, base, l, y, split);
+            }
+        }
     }
 }
 

@@ -569,21 +569,28 @@ extern "C" int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_
 
 // ---------------------------------------------------------------- attention over the cache
 struct KvShape {
-    int rt, row_tiles, splits;
+    int rt, row_tiles;              // sequences of few rows: tiles of 16 rows per wave, row tiles
+    int waves, row_tiles_many;      // sequences of many rows: waves of a workgroup (0: there are none), row tiles
+    int splits;                     // shares of the key axis
 };
+// tiles of 16 rows per wave of the kernel of many rows: what fits the registers
+static constexpr int kv8_rt_many(int bytes, int width) { return bytes == 4 && width == 128 ? 1 : 2; }
 
-// Query rows per wave and how far the key axis is split.  A split costs a second launch (the join, about 2 us), so
-// none has fewer than KV_MIN_TILES tiles, and there are as many as fill the chip about three times over.
+// A split costs a second launch (the join, about 4 us) and the partial results' way out and in, so none has fewer than
+// KV_MIN_TILES tiles, and there are as many as fill the chip about three times over (of few rows: three workgroups
+// fit a CU, of many one of eight waves or two of four).
 static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     KvShape s;
-    const long rows = (long)(d->cu_rows ? d->max_rows : 1) * (d->h / d->hk);
-    const int most = d->dtype == ATHENA_F32 ? (d->width == 128 ? 1 : 2) : d->width == 128 ? 2 : 4;     // what fits the registers
-    s.rt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
-    const long tiles = (rows + 16 * s.rt - 1) / (16 * s.rt);
-    s.row_tiles = (int)(tiles < 65536 ? tiles : 65536);
-    const long units = (long)d->B * d->hk * s.row_tiles, key_tiles = ((long)d->table_width * d->block_size + KV_KEYS - 1) / KV_KEYS;
-    long splits = (1536 + units - 1) / units;
-    const long cap = key_tiles / KV_MIN_TILES;
+    const long G = d->h / d->hk, most = (long)(d->cu_rows ? d->max_rows : 1) * G, few = G > KV_FEW ? G : KV_FEW, rows = most < few ? most : few;
+    s.rt = rows <= 16 || (d->dtype == ATHENA_F32 && d->width == 128) ? 1 : 2;
+    s.row_tiles = (int)((rows + 16 * s.rt - 1) / (16 * s.rt));
+    const int rt = kv8_rt_many(d->dtype == ATHENA_F32 ? 4 : 2, d->width);
+    s.waves = most <= few ? 0 : most > 512 ? 8 : 4;
+    const long tiles = s.waves ? (most + 16 * rt * s.waves - 1) / (16 * rt * s.waves) : 0;
+    s.row_tiles_many = (int)(tiles < 65536 ? tiles : 65536);
+    const long pairs = (long)d->B * d->hk, units = pairs * s.row_tiles, units_many = pairs * s.row_tiles_many * (s.waves / 4);
+    const long key_tiles = ((long)d->table_width * d->block_size + KV_KEYS - 1) / KV_KEYS, cap = key_tiles / KV_MIN_TILES;
+    long splits = s.waves ? (1536 + units_many - 1) / units_many : (1536 + units - 1) / units;
     if (splits > cap) splits = cap;
     s.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
     return s;
@@ -598,12 +605,19 @@ extern "C" int64_t athena_kv8_attention_workspace_bytes(const athena_kv8_attenti
 }
 
 template <typename T, int W>
-static void kv8_launch(const KvAttn& a, const KvShape& sh, hipStream_t s) {
-    const long units = ((long)a.B * a.hk + 7) / 8 * 8 * sh.row_tiles * sh.splits;
-    const dim3 grid((unsigned)units), block(256);
-    if (sh.rt == 4) {
-        if constexpr (W < 128 && sizeof(T) == 2) ATHENA_LAUNCH((kv8_attention_kernel<T, W, 4>), grid, block, 0, s, a);
-    } else if (sh.rt == 2) {
+static void kv8_launch(KvAttn a, const KvShape& sh, hipStream_t s) {
+    const long pairs = ((long)a.B * a.hk + 7) / 8 * 8;
+    const dim3 block(256);
+    if (sh.waves) {
+        a.row_tiles = sh.row_tiles_many;
+        const dim3 grid((unsigned)(pairs * sh.row_tiles_many * sh.splits));
+        constexpr int RT = kv8_rt_many(sizeof(T), W);
+        if (sh.waves == 8) ATHENA_LAUNCH((kv8_attention_rows_kernel<T, W, RT, 8>), grid, dim3(512), 0, s, a);
+        else ATHENA_LAUNCH((kv8_attention_rows_kernel<T, W, RT, 4>), grid, block, 0, s, a);
+    }
+    a.row_tiles = sh.row_tiles;
+    const dim3 grid((unsigned)(pairs * sh.row_tiles * sh.splits));
+    if (sh.rt == 2) {
         if constexpr (W < 128 || sizeof(T) == 2) ATHENA_LAUNCH((kv8_attention_kernel<T, W, 2>), grid, block, 0, s, a);
     } else ATHENA_LAUNCH((kv8_attention_kernel<T, W, 1>), grid, block, 0, s, a);
 }
@@ -625,7 +639,8 @@ extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_s
     ATHENA_REQUIRE(athena_aligned16(d->k_codes) && athena_aligned16(d->v_codes), ATHENA_E_ALIGN,
                    "athena_kv8_attention: codes must lie on 16 bytes");
     const KvShape sh = kv8_shape(d);
-    ATHENA_REQUIRE(((long)B * hk + 7) / 8 * 8 * sh.row_tiles * sh.splits < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: too many workgroups");
+    ATHENA_REQUIRE(((long)B * hk + 7) / 8 * 8 * sh.row_tiles * sh.splits < (1L << 31) &&
+                       ((long)B * hk + 7) / 8 * 8 * sh.row_tiles_many * sh.splits < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: too many workgroups");
     const int64_t need = athena_kv8_attention_workspace_bytes(d);
     ATHENA_REQUIRE(need == 0 || (d->workspace && d->workspace_bytes >= need), ATHENA_E_SHAPE,
                    "athena_kv8_attention: workspace of %ld bytes, %ld needed", (long)d->workspace_bytes, (long)need);
@@ -635,7 +650,7 @@ extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_s
     const int out_wide = (uintptr_t)d->out % (4 * e) == 0 && d->ldo % 4 == 0 && d->ldo_head % 4 == 0;
     KvAttn a = {d->q, d->ldq, d->ldq_head, d->k_codes, d->v_codes, d->k_scale, d->v_scale, d->tables, d->ld_tables, d->lens, d->cu_rows,
                 d->out, d->ldo, d->ldo_head, d->lse, part, part + (sh.splits > 1 ? (long)sh.splits * N * h * d->dk : 0), d->table_width,
-                d->num_blocks, B, N, h, hk, d->dk, d->block_size, d->causal, sh.splits, sh.row_tiles, q_wide, out_wide, d->scale};
+                d->num_blocks, B, N, h, hk, d->dk, d->block_size, __builtin_ctz(d->block_size), d->causal, sh.splits, sh.row_tiles, sh.waves ? (h / hk > KV_FEW ? h / hk : KV_FEW) : 0x7fffffff, q_wide, out_wide, d->scale};
     hipStream_t s = (hipStream_t)stream;
 #define KV_LAUNCH(T)                                      \
     do {                                                  \
