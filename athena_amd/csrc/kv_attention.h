@@ -411,7 +411,7 @@ template <int W> __device__ __forceinline__ int kv_swz(int key) {
 }
 
 template <typename T, int W, int RT, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void kv8_attention_rows_kernel(KvAttn a) {
+__global__ __launch_bounds__(64 * NW, (W < 128 && sizeof(T) == 2 ? 3 : 2)) void kv8_attention_rows_kernel(KvAttn a) {
     constexpr bool TWO = sizeof(T) == 4;
     constexpr int F = W / 32, D = W / 16, NT = 64 * NW, ROWS = 16 * NW * RT, NC = W / 8, PIECES = 4 * W, NP = (PIECES + NT - 1) / NT;
     __shared__ __attribute__((aligned(16))) f16_t s_k[2][64 * W], s_v[2][64 * W];
@@ -499,17 +499,24 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_attention_rows_kernel(KvAttn a
             if (t * KV_KEYS < q.most) {                     // (a causal wave is done before the workgroup's last rows are)
                 // (the XORs depend on the lane alone: everything else is a constant distance from these four places)
                 const f16_t *sk0 = s_k[t & 1] + at_k0, *sk1 = s_k[t & 1] + at_k1, *sv0 = s_v[t & 1] + at_v0, *sv1 = s_v[t & 1] + at_v1;
+                // (fragments are asked for one step ahead, and the compiler is kept from moving the requests down to their use)
                 f32x4_t s[RT][4];
+                f16x8_t kf[2][F];
+#pragma unroll
+                for (int f = 0; f < F; ++f) kf[0][f] = *(const f16x8_t*)((f & 1 ? sk1 : sk0) + (f >> 1) * 64);
 #pragma unroll
                 for (int i4 = 0; i4 < 4; ++i4) {
+                    if (i4 < 3) {
+#pragma unroll
+                        for (int f = 0; f < F; ++f) kf[(i4 + 1) & 1][f] = *(const f16x8_t*)((f & 1 ? sk1 : sk0) + (i4 + 1) * 4 * W + (f >> 1) * 64);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int r = 0; r < RT; ++r) s[r][i4] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int f = 0; f < F; ++f) {
-                        const f16x8_t kf = *(const f16x8_t*)((f & 1 ? sk1 : sk0) + i4 * 4 * W + (f >> 1) * 64);
+                    for (int f = 0; f < F; ++f)
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) q.score(s[r][i4], kf, r, f);
-                    }
+                        for (int r = 0; r < RT; ++r) q.score(s[r][i4], kf[i4 & 1][f], r, f);
                 }
                 const bool whole = !__any(!ok_now) && (t + 1) * KV_KEYS <= q.least;
                 const int j0 = t * KV_KEYS + 16 * g;
@@ -518,14 +525,20 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_attention_rows_kernel(KvAttn a
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
                     x[r].tile(s[r], ks_now * q.qs[r], vs_now, vl, whole, ok_now ? q.limit[r] - j0 : 0, p[r], pl[r]);
+                f16x8_t vf[2][2];
+                vf[0][0] = *(const f16x8_t*)sv0;
+                vf[0][1] = *(const f16x8_t*)sv1;
 #pragma unroll
                 for (int d = 0; d < D; ++d) {
-                    const f16x8_t v0 = *(const f16x8_t*)(sv0 + d * 16 * 64), v1 = *(const f16x8_t*)(sv1 + d * 16 * 64);
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        x[r].add(d, v0, p[r][0], pl[r][0]);
-                        x[r].add(d, v1, p[r][1], pl[r][1]);
+                    if (d + 1 < D) {
+                        vf[(d + 1) & 1][0] = *(const f16x8_t*)(sv0 + (d + 1) * 16 * 64);
+                        vf[(d + 1) & 1][1] = *(const f16x8_t*)(sv1 + (d + 1) * 16 * 64);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) x[r].add(d, vf[d & 1][0], p[r][0], pl[r][0]);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) x[r].add(d, vf[d & 1][1], p[r][1], pl[r][1]);
                 }
             }
             if (next) stage((t + 1) & 1);
