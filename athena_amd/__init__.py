@@ -11,6 +11,7 @@ from .models.mtl_seq2seq import MtlTransformerCtc
 from .models.speech_transformer import SpeechTransformer
 from .solver import BaseSolver, DecoderSolver, HorovodSolver
 from .tools.beam_search import BeamSearchDecoder
+from .tools.cached_decode import CachedPropagate, LogitRules
 from .tools.ctc_scorer import CTCPrefixScorer
 from .utils.checkpoint import Checkpoint
 from .utils.hparam import HParams, register_and_parse_hparams
@@ -22,7 +23,7 @@ from .utils.misc import (create_multihead_mask, generate_square_subsequent_mask,
 __all__ = [
     "CTCLoss", "MPCLoss", "MaskedPredictCoding", "DeepSpeechModel", "Seq2SeqSparseCategoricalCrossentropy", "Accuracy", "CharactorAccuracy", "CTCAccuracy",
     "Seq2SeqSparseCategoricalAccuracy", "BaseModel", "MtlTransformerCtc", "SpeechTransformer", "BaseSolver",
-    "HorovodSolver", "DecoderSolver", "BeamSearchDecoder", "CTCPrefixScorer", "HParams", "register_and_parse_hparams", "ExponentialDecayAdam", "WarmUpAdam",
+    "HorovodSolver", "DecoderSolver", "BeamSearchDecoder", "CTCPrefixScorer", "CachedPropagate", "LogitRules", "HParams", "register_and_parse_hparams", "ExponentialDecayAdam", "WarmUpAdam",
     "WarmUpLearningSchedule", "MetricChecker", "set_default_summary_writer", "create_multihead_mask",
     "generate_square_subsequent_mask", "insert_eos_in_labels", "insert_sos_in_labels", "validate_seqs",
     "Checkpoint",

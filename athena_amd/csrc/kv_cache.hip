@@ -593,7 +593,7 @@ static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     s.row_tiles_many = (int)(tiles < 65536 ? tiles : 65536);
     const long pairs = (long)d->B * d->hk, units = pairs * s.row_tiles, units_many = pairs * s.row_tiles_many * (s.waves / 4);
     const long key_tiles = ((long)d->table_width * d->block_size + KV_KEYS - 1) / KV_KEYS, cap = key_tiles / KV_MIN_TILES;
-    long splits = s.waves ? (1536 - 1 + units_many - 1) / units_many : (1535 + units) / units;
+    long splits = s.waves ? (1535 + units_many) / units_many : (1535 + units) / units;
     if (splits > cap) splits = cap;
     s.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
     return s;

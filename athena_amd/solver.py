@@ -703,18 +703,25 @@ class DecoderSolver(BaseSolver):
         "min_active": 0,
         "wfst_beam": 30.0,
         "max_seq_len": 100,
-        "wfst_graph": None
+        "wfst_graph": None,
+        # not in the reference: keys and values of the history kept in 8 bits instead of computed again at
+        # every step, and penalties for repeated labels (1, 0, 0: none)
+        "kv_cache": False,
+        "repetition_penalty": 1.0,
+        "presence_penalty": 0.0,
+        "frequency_penalty": 0.0
     }
 
     def __init__(self, model, data_descriptions=None, config=None):
         from .tools.beam_search import BeamSearchDecoder
+        from .tools.cached_decode import CachedPropagate
         from .utils.hparam import register_and_parse_hparams
         self.model = model
         self.optimizer = None
         self.hparams = register_and_parse_hparams(self.default_config, config, cls=self.__class__)
         if self.hparams.decoder_type == "beam_search_decoder":
-            self.decoder = BeamSearchDecoder.build_decoder(self.hparams, model.num_class, model.sos, model.eos,
-                                                           model.time_propagate)
+            step = CachedPropagate(model, self.hparams.beam_size) if self.hparams.kv_cache else model.time_propagate
+            self.decoder = BeamSearchDecoder.build_decoder(self.hparams, model.num_class, model.sos, model.eos, step)
         elif self.hparams.decoder_type == "wfst_decoder":
             raise NotImplementedError("the WFST decoder (athena/tools/wfst_decoder.py) is not built")
         else:

@@ -11,6 +11,7 @@ import collections
 import numpy as np
 import torch
 
+from .cached_decode import LogitRules
 from .ctc_scorer import CTCPrefixScorer
 
 CandidateHolder = collections.namedtuple(
@@ -76,6 +77,7 @@ class BeamSearchDecoder:
         self.lm_model = None
         self.states = []
         self.decoder_one_step = None
+        self.logit_rules = None
 
     @staticmethod
     def build_decoder(hparams, num_class, sos, eos, decoder_one_step, lm_model=None):
@@ -84,6 +86,10 @@ class BeamSearchDecoder:
         beam = hparams.decoder_type == "beam_search_decoder"
         dec = BeamSearchDecoder(num_class, sos, eos, beam_size=hparams.beam_size if beam else 1)
         dec.decoder_one_step = decoder_one_step
+        rules = LogitRules(getattr(hparams, "repetition_penalty", 1.0), getattr(hparams, "presence_penalty", 0.0),
+                           getattr(hparams, "frequency_penalty", 0.0))
+        if rules:
+            dec.set_logit_rules(rules)
         if beam and hparams.ctc_weight != 0:
             dec.set_ctc_scorer(CTCPrefixScorer(eos, ctc_beam=hparams.beam_size * 2, num_classes=num_class,
                                                ctc_weight=hparams.ctc_weight))
@@ -104,12 +110,18 @@ class BeamSearchDecoder:
         self.ctc_scorer = ctc_scorer
         self.scorers.append(ctc_scorer)
 
+    def set_logit_rules(self, rules):
+        """Penalties, biases or a grammar on the logits of every step (``LogitRules``)."""
+        self.logit_rules = rules
+
     def beam_search_score(self, candidate_holder, encoder_outputs):
         """One decoder step on every live hypothesis: scores [n, num_class] of extending it by each
         class (beam_search.py:120-150)."""
         logits, history, states = self.decoder_one_step(candidate_holder.cand_logits, candidate_holder.cand_seqs,
                                                         self.states, encoder_outputs)
         self.states = states
+        if self.logit_rules is not None:
+            logits = self.logit_rules(logits, candidate_holder.cand_seqs)
         logprobs = torch.log_softmax(logits.to(torch.float32), dim=-1).cpu().numpy().astype(np.float32)
         new_scores = logprobs + candidate_holder.cand_scores[:, None].astype(np.float32)
         new_states = candidate_holder.cand_states
@@ -132,6 +144,8 @@ class BeamSearchDecoder:
             self.lm_model.reset()
         enc, enc_mask = encoder_outputs
         max_seq_len = enc.shape[1]
+        if hasattr(self.decoder_one_step, "begin"):        # a step with a cache takes the encoder output once
+            self.decoder_one_step.begin(enc, enc_mask)
         done = _Finished(self.beam_size, max_seq_len, self.eos)
         open_classes = np.array([c for c in range(self.num_class) if c != self.eos])
         for pos in range(max_seq_len):

@@ -140,3 +140,30 @@ def test_oracle_append_grows_a_scale():
     ok.append(torch.tensor([[[254.0, 3.0, -3.0]]]), [1], codes, scale)
     assert float(scale) == 2.0 and codes[0, 0, 0, :4].tolist() == [64, -32, 0, 0]
     assert codes[0, 0, 1, :4].tolist() == [127, 2, -2, 0]                     # 1.5 rounds to the even 2
+
+
+def test_pack_classes():
+    from athena_amd.tools import pack_classes
+    import numpy as np
+    allowed = np.zeros((2, 40), dtype=bool)
+    allowed[0, [0, 31, 32, 39]] = True
+    words = pack_classes(allowed)
+    assert words.dtype == torch.int32 and tuple(words.shape) == (2, 2)
+    assert words[0].tolist() == [1 - 2 ** 31, 1 | 1 << 7] and words[1].tolist() == [0, 0]
+    with pytest.raises(ValueError):
+        pack_classes(allowed[0])
+
+
+def test_logit_rules_are_off_by_default():
+    from athena_amd import LogitRules
+    from athena_amd.solver import DecoderSolver
+    from athena_amd.tools import BeamSearchDecoder
+    from athena_amd.utils.hparam import register_and_parse_hparams
+    assert not LogitRules() and LogitRules(repetition=1.2) and LogitRules(bias={3: 1.0}) and LogitRules(grammar=lambda s: None)
+    with pytest.raises(ValueError):
+        LogitRules(repetition=0)
+    hp = register_and_parse_hparams(DecoderSolver.default_config, {"decoder_type": "beam_search_decoder"})
+    assert hp.kv_cache is False
+    assert BeamSearchDecoder.build_decoder(hp, 4, 3, 3, lambda *a: None).logit_rules is None
+    hp.frequency_penalty = 0.5
+    assert BeamSearchDecoder.build_decoder(hp, 4, 3, 3, lambda *a: None).logit_rules.frequency == 0.5
