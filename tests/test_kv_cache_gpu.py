@@ -375,6 +375,44 @@ def test_attention_over_long_contexts(h, hk, dk, bs, n):
             assert bool((err <= 0).all()), (b, g, float(err.max()))
 
 
+def _dense_reference(q, cache, tables, lens, cu, causal, scale):
+    """(out, spread) in 64 bits on the GPU, sequence by sequence and head by head."""
+    n, h, dk = q.shape
+    hk, bs, w = cache[0].shape[1:]
+    put = [t.to(dev()) for t in (q, *cache)]
+    q, kc, vc, ks, vs = put
+    out, spread = torch.zeros(n, h, dk, dtype=torch.float64, device=dev()), torch.zeros(n, h, dk, dtype=torch.float64, device=dev())
+    for b, m in enumerate(lens):
+        blocks = tables[b, :-(-m // bs)].long().to(dev())
+        lo, hi = cu[b], cu[b + 1]
+        place = m - (hi - lo) + torch.arange(hi - lo, device=dev()) if causal else torch.full((hi - lo,), m - 1, device=dev())
+        hidden = torch.arange(m, device=dev())[None] > place[:, None]
+        for i in range(h):
+            g = i // (h // hk)
+            k = (kc[blocks, g].double() * ks[blocks, g].double()[:, None, None]).reshape(-1, w)[:m, :dk]
+            v = (vc[blocks, g].double() * vs[blocks, g].double()[:, None, None]).transpose(1, 2).reshape(-1, w)[:m, :dk]
+            p = torch.softmax((q[lo:hi, i].double() @ k.t() * scale).masked_fill(hidden, -math.inf), -1)
+            out[lo:hi, i], spread[lo:hi, i] = p @ v, p @ v.abs()
+    return out.cpu(), spread.cpu()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("h,hk,dk,bs,lens,rows", [
+    (8, 2, 128, 64, [3001, 700], [301, 130]),               # rows by the hundreds, the key axis split there too
+    (4, 4, 64, 16, [1500, 1201, 65], [1500, 66, 65]),
+    (6, 1, 24, 32, [900, 2500], [11, 200]),
+    (8, 2, 128, 128, [5000, 40, 2300, 1], [1, 40, 300, 1]),  # single rows beside chunks
+    (40, 1, 80, 16, [2100, 2100], [1, 9])])                 # one kv head for forty: a single token is forty rows
+def test_attention_of_hundreds_of_rows(dtype, causal, h, hk, dk, bs, lens, rows):
+    q, cache, tables, cu = _attention_case(sum(lens), lens, rows, h, hk, dk, bs, dtype)
+    got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=_i32(cu),
+                            max_rows=max(rows), causal=causal).cpu().double()
+    want, spread = _dense_reference(q, cache, tables, lens, cu, causal, 1 / math.sqrt(dk))
+    err = (got - want).abs() - _bound(dtype, q, cache, spread, want, 1 / math.sqrt(dk))
+    assert bool((err <= 0).all()), float(err.max())
+
+
 def test_attention_offsets_beyond_32_bits():
     """A pool of more than 2^32 bytes: blocks at its far end."""
     nb, hk, bs, w = 4 * 1024 + 8, 16, 128, 128              # 1.05 GiB of codes each for 4104 blocks ...
