@@ -1334,16 +1334,20 @@ def kv_plan(lens, new_rows, tables, free_blocks, free_count, block_size, rows, i
     if rows < 0:
         _refuse("kv_plan", "room for %d rows", rows)
     stream = _here("kv_plan", lens, new_rows, tables, free_blocks, free_count)
-    # one piece of memory for everything the plan writes afresh
-    sizes = (B + 1, rows, rows, 4, 0 if in_place else B, 0 if in_place else 1, 3 * B + 3)
-    cu, slots, positions, status, out, count, work = torch.empty(sum(sizes), dtype=_I32, device=lens.device).split(sizes)
-    if in_place:
-        out, count = lens, free_count
+    # one piece of memory for everything the plan writes afresh; what the caller does not get to see lies at its end
+    sizes = [B + 1, rows, rows, 4] + ([] if in_place else [B, 1]) + [3 * B + 3]
+    fresh = torch.empty(sum(sizes), dtype=_I32, device=lens.device)
+    parts = fresh.split_with_sizes(sizes)
+    at = fresh.data_ptr()
+    p_slots, p_positions, p_status = at + 4 * (B + 1), at + 4 * (B + 1 + rows), at + 4 * (B + 1 + 2 * rows)
+    out, count = (lens, free_count) if in_place else parts[4:6]
+    p_lens, p_count = lens.data_ptr(), free_count.data_ptr()
+    p_work = p_status + 16 if in_place else p_status + 16 + 4 * (B + 1)
     _lib.check(_lib.load().athena_kv_plan(_lib.KvPlanDesc.pack(
-        lens.data_ptr(), new_rows.data_ptr(), tables.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(), cu.data_ptr(),
-        slots.data_ptr(), positions.data_ptr(), out.data_ptr(), count.data_ptr(), status.data_ptr(), work.data_ptr(),
+        p_lens, new_rows.data_ptr(), tables.data_ptr(), free_blocks.data_ptr(), p_count, at, p_slots, p_positions,
+        p_lens if in_place else p_status + 16, p_count if in_place else p_status + 16 + 4 * B, p_status, p_work,
         ldt if B > 1 else width, width, free_blocks.numel(), B, block_size, rows, 0), stream), "athena_kv_plan")
-    return KvPlan(cu, slots, positions, out, count, status)
+    return KvPlan(parts[0], parts[1], parts[2], out, count, parts[3])
 
 
 def _kv8_cache(name, k_codes, v_codes, k_scale, v_scale):
@@ -1355,7 +1359,7 @@ def _kv8_cache(name, k_codes, v_codes, k_scale, v_scale):
     nb, hk, bs, w = shape
     if v_codes.shape != (nb, hk, w, bs):
         _refuse(name, "v_codes must be [%d, %d, %d, %d]", nb, hk, w, bs)
-    if k_scale.dtype is not _FP32 or v_scale.dtype is not _FP32 or k_scale.shape != (nb, hk) or v_scale.shape != (nb, hk) or \
+    if k_scale.dtype is not _FP32 or v_scale.dtype is not _FP32 or k_scale.numel() != nb * hk or v_scale.numel() != nb * hk or \
             not k_scale.is_contiguous() or not v_scale.is_contiguous():
         _refuse(name, "scales must be contiguous fp32 [%d, %d]", nb, hk)
     return nb, hk, bs, w
@@ -1405,7 +1409,7 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows=N
     else:
         _int_vector("kv8_attention", "cu_rows", cu_rows, B + 1)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         so = (h * dk, dk)
     else:
         o_shape, so = _head_rows("kv8_attention", "out", out)
@@ -1487,7 +1491,7 @@ def logits_process(logits, history=None, history_len=None, repetition=None, pres
     if allowed is not None:
         lda = _row_matrix(name, "allowed", allowed, _I32, R, (V + 31) // 32)
     if out is None:
-        out, ldo = torch.empty(shape, dtype=logits.dtype, device=logits.device), V
+        out, ldo = torch.empty_like(logits, memory_format=torch.contiguous_format), V
     else:
         so = out.stride()
         if out.shape != shape or out.dtype != logits.dtype or (so[1] != 1 and V > 1):
