@@ -7,8 +7,9 @@
 // A workgroup takes one tile of classes of one row.  Its logits are requested first; while they travel, occurrences of
 // the tile's classes are counted in LDS from the history (whole-number atomics: their order does not matter) and classes with
 // a bias of their own get a flag in the counter's top bit.  Then the tile passes once, 16 bytes a lane.  Bound by the
-// logits' way in and out; the history is read again by every tile of a row, from the L2, so tiles are large (8192) where
-// there are enough of them to fill the chip and 1024 (fp32) / 2048 (bf16) where there are not.
+// logits' way in and out; the history is read again by every tile of a row, from the L2, so tiles are large (4096: 16 KB of
+// counters, eight workgroups a CU; 8192 took 57 us where 4096 take 43) where there are enough of them to fill the chip, and
+// 1024 (fp32) / 2048 (bf16) where there are not.
 struct LogitsArgs {
     const void* logits;
     void* out;
@@ -20,6 +21,13 @@ struct LogitsArgs {
 
 #define LOGITS_BIASED 0x80000000u
 #define LOGITS_LIST 256         // biases of one tile kept in LDS; more are looked up in memory
+
+// Where the counter of a tile's class i lies: a thread reads E of them, four at a time, and the fours that are read
+// together stand side by side.
+template <int E, int TILE>
+__device__ __forceinline__ unsigned logits_place(unsigned i) {
+    return E == 8 ? (i >> 3) * 4 + (i & 3) + ((i >> 2) & 1) * (TILE / 2) : i;
+}
 
 // NB vectors of 16 bytes per thread
 template <typename T, int NB>
@@ -54,7 +62,7 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
 #pragma unroll 4
         for (int i = tid; i < n; i += 256) {
             const unsigned at = (unsigned)ids[i] - (unsigned)v0;
-            if (at < (unsigned)nv) atomicAdd(&count[at], 1u);
+            if (at < (unsigned)nv) atomicAdd(&count[logits_place<E, TILE>(at)], 1u);
         }
     }
     if (tid < 64) {                             // the tile's own biases, in their order
@@ -64,7 +72,7 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
             const unsigned at = j < a.nb ? (unsigned)a.bias_ids[(long)r * a.ld_bias_ids + j] - (unsigned)v0 : ~0u;
             const unsigned long long found = __ballot(at < (unsigned)nv);
             if (at < (unsigned)nv) {
-                atomicOr(&count[at], LOGITS_BIASED);
+                atomicOr(&count[logits_place<E, TILE>(at)], LOGITS_BIASED);
                 const int k = n + __popcll(found & ((1ull << tid) - 1));
                 if (k < LOGITS_LIST) {
                     list_at[k] = at;
@@ -83,27 +91,41 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
     for (int b = 0; b < NB; ++b) {
         const int i = (b * 256 + tid) * E;
         if (i >= nv) continue;
+        unsigned c[E], any = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int v = v0 + i + e;
-            const unsigned c = count[i + e], n = c & ~LOGITS_BIASED;
-            float y = to_f32<T>(x[b].e[e]);
-            if (n) {
-                y = y > 0.f ? y / rep : y * rep;
-                y = y - freq * (float)n - pres;
-            }
-            if (a.bias && i + e < nv) y += a.bias[(long)r * a.ld_bias + v];
-            if (c & LOGITS_BIASED) {
-                float own = 0.f;                // entries of one class add up in their order
-                if (biased <= LOGITS_LIST) {
-                    for (int j = 0; j < biased; ++j) own += list_at[j] == (unsigned)(i + e) ? list_value[j] : 0.f;
-                } else {
-                    for (int j = 0; j < a.nb; ++j)
-                        if (a.bias_ids[(long)r * a.ld_bias_ids + j] == v) own += a.bias_values[(long)r * a.ld_bias_values + j];
+        for (int q = 0; q < E; q += 4) {
+            const uint4 four = *(const uint4*)&count[logits_place<E, TILE>(i + q)];
+            c[q] = four.x, c[q + 1] = four.y, c[q + 2] = four.z, c[q + 3] = four.w;
+            any |= (four.x | four.y) | (four.z | four.w);
+        }
+        if (any || a.bias) {                    // (most vectors hold no class of the history and none with a bias)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int v = v0 + i + e;
+                const unsigned n = c[e] & ~LOGITS_BIASED;
+                float y = to_f32<T>(x[b].e[e]);
+                if (n) {
+                    y = y > 0.f ? y / rep : y * rep;
+                    y = y - freq * (float)n - pres;
                 }
-                y += own;
+                if (a.bias && i + e < nv) y += a.bias[(long)r * a.ld_bias + v];
+                if (c[e] & LOGITS_BIASED) {
+                    float own = 0.f;            // entries of one class add up in their order
+                    if (biased <= LOGITS_LIST) {
+                        for (int j = 0; j < biased; ++j) own += list_at[j] == (unsigned)(i + e) ? list_value[j] : 0.f;
+                    } else {
+                        for (int j = 0; j < a.nb; ++j)
+                            if (a.bias_ids[(long)r * a.ld_bias_ids + j] == v) own += a.bias_values[(long)r * a.ld_bias_values + j];
+                    }
+                    y += own;
+                }
+                x[b].e[e] = from_f32<T>(y);
             }
-            x[b].e[e] = from_f32<T>((mask[b] >> (v & 31)) & 1u ? y : -INFINITY);
+        }
+        if (mask[b] != ~0u) {
+            const unsigned bits = mask[b] >> ((v0 + i) & 31);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[b].e[e] = (bits >> e) & 1u ? x[b].e[e] : from_f32<T>(-INFINITY);
         }
         if (a.wide && i + E <= nv) *(Vec*)(out + i) = x[b];
         else {
@@ -129,15 +151,15 @@ extern "C" int athena_logits_process(const athena_logits_desc* d, athena_stream_
                     d->ld_allowed, R, V, d->history ? d->L : 0, d->nb, 0};
     const int e = d->dtype == ATHENA_BF16 ? 2 : 4;
     a.wide = athena_aligned16(d->logits) && athena_aligned16(d->out) && (R == 1 || (d->ldl * e % 16 == 0 && d->ldo * e % 16 == 0));
-    const bool large = (long)R * ((V + 8191) / 8192) >= 512;
-    const int tile = large ? 8192 : 4096 / e;
+    const bool large = (long)R * ((V + 4095) / 4096) >= 512;
+    const int tile = large ? 4096 : 4096 / e;
     const dim3 grid((V + tile - 1) / tile, R);
     hipStream_t s = (hipStream_t)stream;
     if (d->dtype == ATHENA_BF16) {
-        if (large) ATHENA_LAUNCH((logits_process_kernel<bf16_t, 4>), grid, dim3(256), 0, s, a);
+        if (large) ATHENA_LAUNCH((logits_process_kernel<bf16_t, 2>), grid, dim3(256), 0, s, a);
         else ATHENA_LAUNCH((logits_process_kernel<bf16_t, 1>), grid, dim3(256), 0, s, a);
     } else {
-        if (large) ATHENA_LAUNCH((logits_process_kernel<float, 8>), grid, dim3(256), 0, s, a);
+        if (large) ATHENA_LAUNCH((logits_process_kernel<float, 4>), grid, dim3(256), 0, s, a);
         else ATHENA_LAUNCH((logits_process_kernel<float, 1>), grid, dim3(256), 0, s, a);
     }
     ATHENA_CHECK_LAUNCH("athena_logits_process");
