@@ -147,7 +147,7 @@ template <typename T, int W, int RT> struct KvQueries {
     }
 };
 
-// One tile of 64 keys of one tile of 16 rows: the running maxima and sum, and probability times value scale as operands.
+// One tile of 16 rows: the running maxima, the sum of exponentials and the sums of values.
 // ``ksq`` (not negative) brings scores to exponents of two, ``vs`` is the lane's value scale, ``vl`` its logarithm to base 2.
 template <int W, bool TWO> struct KvSoftmax {
     f32x4_t o[W / 16];
@@ -158,7 +158,9 @@ template <int W, bool TWO> struct KvSoftmax {
 #pragma unroll
         for (int d = 0; d < W / 16; ++d) o[d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ void tile(f32x4_t (&s)[4], float ksq, float vs, float vl, bool whole, int seen, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
+    // Steps of a tile; each is called for all of a wave's row tiles before the next, so that their chains of dependent
+    // instructions run side by side.  1: the new maxima
+    __device__ __forceinline__ void peak(f32x4_t (&s)[4], float ksq, float vl, bool whole, int seen, float& mn, float& mn2) {
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -172,45 +174,54 @@ template <int W, bool TWO> struct KvSoftmax {
             for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
         // (a scale of 0 beside a score of -inf, which is "hidden": still hidden)
         top = top == -INFINITY ? top : top * ksq;
-        const float mn = fmaxf(m, rows4_max(top)), mn2 = fmaxf(m2, rows4_max(top + vl));
-        const float base = mn == -INFINITY ? 0.f : mn, base2 = mn2 == -INFINITY ? 0.f : mn2;
-        if (__any(mn > m || mn2 > m2)) {
-            l *= __builtin_amdgcn_exp2f(m - base);
-            const float down = __builtin_amdgcn_exp2f(m2 - base2);
+        mn = fmaxf(m, rows4_max(top));
+        mn2 = fmaxf(m2, rows4_max(top + vl));
+    }
+    // 2: what is there already, relative to them
+    __device__ __forceinline__ void rescale(float mn, float mn2) {
+        l *= __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        const float down = __builtin_amdgcn_exp2f(m2 - (mn2 == -INFINITY ? 0.f : mn2));
 #pragma unroll
-            for (int d = 0; d < W / 16; ++d)
+        for (int d = 0; d < W / 16; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[d][e] *= down;
-            m = mn;
-            m2 = mn2;
-        }
-        // Probability times value scale in one exponential, and the sum of the lane's sixteen divided by the scale again.
-        // Where the scale is far below the largest product so far (or 0, or not finite) that division would lose the
-        // probabilities: they are then worked out by themselves.
-        const float shift = vl + base - base2;
-        if (whole && !__any(!(shift > -40.f))) {
-            const float at = vl - base2;
-            float sum = 0.f;
+            for (int e = 0; e < 4; ++e) o[d][e] *= down;
+        m = mn;
+        m2 = mn2;
+    }
+    // Probability times value scale in one exponential, and the sum of the lane's sixteen divided by the scale again.
+    // Where the scale is far below the largest product so far (or 0, or not finite) that division would lose the
+    // probabilities: they are then worked out by themselves (weigh_apart).
+    __device__ __forceinline__ float shift(float vl) const { return vl + (m == -INFINITY ? 0.f : m) - (m2 == -INFINITY ? 0.f : m2); }
+    // 3: probabilities times value scales
+    __device__ __forceinline__ void weigh(f32x4_t (&s)[4], float ksq, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
+        const float at = vl - m2;
+        float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, at));
-                    sum += s[i][e];
-                }
-            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
-        } else {                                            // scales that are 0 or not finite must not reach hidden keys
-            const float vf = fminf(vs * __builtin_amdgcn_exp2f(base - base2), 3.4e38f);
+            for (int e = 0; e < 4; ++e) {
+                s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, at));
+                sum += s[i][e];
+            }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift(vl)), l);
+        pack(s, p, pl);
+    }
+    __device__ __forceinline__ void weigh_apart(f32x4_t (&s)[4], float ksq, float vs, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
+        // scales that are 0 or not finite must not reach hidden keys
+        const float base = m == -INFINITY ? 0.f : m, base2 = m2 == -INFINITY ? 0.f : m2;
+        const float vf = fminf(vs * __builtin_amdgcn_exp2f(base - base2), 3.4e38f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool hidden = s[i][e] == -INFINITY;
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, -base));
-                    l += hidden ? 0.f : x;
-                    s[i][e] = hidden ? 0.f : x * vf;
-                }
-        }
+            for (int e = 0; e < 4; ++e) {
+                const bool hidden = s[i][e] == -INFINITY;
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, -base));
+                l += hidden ? 0.f : x;
+                s[i][e] = hidden ? 0.f : x * vf;
+            }
+        pack(s, p, pl);
+    }
+    __device__ __forceinline__ void pack(const f32x4_t (&s)[4], f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -225,6 +236,34 @@ template <int W, bool TWO> struct KvSoftmax {
         if (TWO) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[d], 0, 0, 0);
     }
 };
+
+// The softmax's part of one tile of keys, for all row tiles of a wave.
+template <typename T, int W, int RT>
+__device__ __forceinline__ void kv_weights(const KvQueries<T, W, RT>& q, KvSoftmax<W, sizeof(T) == 4> (&x)[RT], f32x4_t (&s)[RT][4], float ks,
+                                           float vs, bool ok, bool whole, int j0, f16x8_t (&p)[RT][2], f16x8_t (&pl)[RT][2]) {
+    const float vl = __builtin_amdgcn_logf(fabsf(vs));      // log2
+    float mn[RT], mn2[RT];
+    bool grown = false;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        x[r].peak(s[r], ks * q.qs[r], vl, whole, ok ? q.limit[r] - j0 : 0, mn[r], mn2[r]);
+        grown = grown || mn[r] > x[r].m || mn2[r] > x[r].m2;
+    }
+    if (__any(grown)) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) x[r].rescale(mn[r], mn2[r]);
+    }
+    bool far = false;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) far = far || !(x[r].shift(vl) > -40.f);
+    if (whole && !__any(far)) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) x[r].weigh(s[r], ks * q.qs[r], vl, p[r], pl[r]);
+    } else {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) x[r].weigh_apart(s[r], ks * q.qs[r], vs, p[r], pl[r]);
+    }
+}
 
 // rows of a sequence that the kernel of few rows takes; the others go to the kernel of many
 __device__ __forceinline__ bool kv_few(const KvAttn& a, int n) { return (long)n * (a.h / a.hk) <= a.few; }
@@ -342,11 +381,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
             if (next) load_keys(t + 4);
             const bool whole = !__any(!ok_now) && (t + 1) * KV_KEYS <= q.least;
             const int j0 = t * KV_KEYS + vc;
-            const float vl = __builtin_amdgcn_logf(fabsf(vs_now));          // log2
             f16x8_t p[RT][2], pl[RT][2];
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-                x[r].tile(s[r], ks_now * q.qs[r], vs_now, vl, whole, ok_now ? q.limit[r] - j0 : 0, p[r], pl[r]);
+            kv_weights<T, W, RT>(q, x, s, ks_now, vs_now, ok_now, whole, j0, p, pl);
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 const f16x8_t v0 = kv_widen(v[d].x, v[d].y), v1 = kv_widen(v[d].z, v[d].w);
@@ -520,11 +556,8 @@ __global__ __launch_bounds__(64 * NW, (W < 128 && sizeof(T) == 2 ? 3 : 2)) void 
                 }
                 const bool whole = !__any(!ok_now) && (t + 1) * KV_KEYS <= q.least;
                 const int j0 = t * KV_KEYS + 16 * g;
-                const float vl = __builtin_amdgcn_logf(fabsf(vs_now));      // log2
                 f16x8_t p[RT][2], pl[RT][2];
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-                    x[r].tile(s[r], ks_now * q.qs[r], vs_now, vl, whole, ok_now ? q.limit[r] - j0 : 0, p[r], pl[r]);
+                kv_weights<T, W, RT>(q, x, s, ks_now, vs_now, ok_now, whole, j0, p, pl);
                 f16x8_t vf[2][2];
                 vf[0][0] = *(const f16x8_t*)sv0;
                 vf[0][1] = *(const f16x8_t*)sv1;
