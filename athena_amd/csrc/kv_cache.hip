@@ -654,7 +654,8 @@ extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_s
     const int out_wide = (uintptr_t)d->out % (4 * e) == 0 && d->ldo % 4 == 0 && d->ldo_head % 4 == 0;
     KvAttn a = {d->q, d->ldq, d->ldq_head, d->k_codes, d->v_codes, d->k_scale, d->v_scale, d->tables, d->ld_tables, d->lens, d->cu_rows,
                 d->out, d->ldo, d->ldo_head, d->lse, part, part + (sh.splits > 1 ? (long)sh.splits * N * h * d->dk : 0), d->table_width,
-                d->num_blocks, B, N, h, hk, d->dk, d->block_size, __builtin_ctz(d->block_size), d->causal, sh.splits, sh.row_tiles, sh.waves ? (h / hk > KV_FEW ? h / hk : KV_FEW) : 0x7fffffff, q_wide, out_wide, d->scale};
+                d->num_blocks, B, N, h, hk, d->dk, d->block_size, __builtin_ctz(d->block_size), d->causal, sh.splits, sh.row_tiles, sh.waves ? (h / hk > KV_FEW ? h / hk : KV_FEW) : 0x7fffffff,
+                ((long)B * hk + 7) / 8 * d->table_width * d->block_size * 2 * d->width <= (4L << 20), q_wide, out_wide, d->scale};
     hipStream_t s = (hipStream_t)stream;
 #define KV_LAUNCH(T)                                      \
     do {                                                  \
