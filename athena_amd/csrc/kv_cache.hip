@@ -286,18 +286,21 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
     const int step = 16 * SUB, begin = first & ~15, end = first + n;
     const float s0 = first == 0 ? 0.f : a.scale[at];
     struct alignas(2 * sizeof(T)) Pair { T e[2]; };
-    Pair raw[16];                                           // two columns of 16 places, where all of the wave's are in the run
-    const auto full = [&](int base) { return pairs && base >= first && base + step <= end; };
+    // Runs of more than a few rows: two columns of 16 places at once, all requests out before the first is waited for.  Places
+    // outside the run read the run's nearest row (which leaves the largest magnitude as it is) and are not written.
+    const bool fast = pairs && n > 4;
+    Pair raw[16];
     auto load = [&](int base) {
-        unsigned off = ((base - first + 16 * sub) * ld + (c < dk ? c : 0)) * (unsigned)sizeof(T);
+        const int r0 = base + 16 * sub - first;
+        const unsigned col = (c < dk ? c : 0) * (unsigned)sizeof(T), pitch = ld * (unsigned)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < 16; ++i, off += ld * (unsigned)sizeof(T)) raw[i] = *(const Pair*)((const char*)x + off);
+        for (int i = 0; i < 16; ++i) raw[i] = *(const Pair*)((const char*)x + (min(max(r0 + i, 0), n - 1) * pitch + col));
         if (c >= dk) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) raw[i].e[0] = raw[i].e[1] = from_f32<T>(0.f);
         }
     };
-    // elsewhere (the ends of a run, single rows): four places at a time, each looked at by itself
+    // others (single rows, odd columns): four places at a time, each looked at by itself
     auto load4 = [&](int p0, float (&f)[4][2]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -314,7 +317,7 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
     if (straight) {
 #pragma unroll 1
         for (int base = begin + rank * step; base < end; base += team * step) {
-            if (full(base)) {
+            if (fast) {
                 load(base);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = max(top, max(mag(to_f32<T>(raw[i].e[0])), mag(to_f32<T>(raw[i].e[1]))));
@@ -372,9 +375,10 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
     if (straight) {
 #pragma unroll 1
         for (int base = begin + rank * step; base < end; base += team * step) {
-            if (full(base) && !tiny) {
+            if (fast && !tiny) {
                 if (end - begin > team * step) load(base);  // (otherwise the registers hold the rows still)
                 const int p0 = base + 16 * sub;
+                const bool whole = p0 >= first && p0 + 16 <= end;
                 unsigned w[2][4];                           // codes of a column, four places to a word
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
@@ -389,13 +393,21 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            *(uint16_t*)(codes + (p0 + 4 * g + i) * W + c) = (uint16_t)__builtin_amdgcn_perm(q[i][1], q[i][0], 0x0c0c0400u);
+                            if (whole || (p0 + 4 * g + i >= first && p0 + 4 * g + i < end))
+                                *(uint16_t*)(codes + (p0 + 4 * g + i) * W + c) = (uint16_t)__builtin_amdgcn_perm(q[i][1], q[i][0], 0x0c0c0400u);
                     }
                 }
                 if (VALUES) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        *(uint4*)(codes + (c + k) * block_size + p0) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+                    for (int k = 0; k < 2; ++k) {
+                        int8_t* p = codes + (c + k) * block_size + p0;
+                        if (whole) *(uint4*)p = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+                        else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (p0 + i >= first && p0 + i < end) p[i] = (int8_t)(w[k][i >> 2] >> (8 * (i & 3)));
+                        }
+                    }
                 }
             } else {
 #pragma unroll 1
