@@ -93,14 +93,14 @@ template <typename T, int W, int RT> struct KvQueries {
     f16x8_t q[RT][F], ql[TWO ? RT : 1][TWO ? F : 1];
     float qs[RT];
     int limit[RT], least, most;                             // of a lane's rows; the fewest and the most of the wave's
-    __device__ __forceinline__ void load(const KvAttn& a, int kvh, int G, int lo, int n, int len, long row0, int qc, int g) {
+    __device__ __forceinline__ void load(const KvAttn& a, int kvh, int G, int lo, int n, int len, int row0, int qc, int g) {
         least = 0x7fffffff;
         most = 0;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const long row = row0 + 16 * r + qc;
-            const bool in = row < (long)n * G;
-            const int token = in ? (int)(row / G) : 0, head = kvh * G + (in ? (int)(row % G) : 0);
+            const int row = row0 + 16 * r + qc;
+            const bool in = row < n * G;
+            const int token = in ? row / G : 0, head = kvh * G + (in ? row - token * G : 0);
             limit[r] = !in ? 0 : a.causal ? min(max(len - n + token + 1, 0), len) : len;
             const T* p = (const T*)a.q + (long)(lo + token) * a.ldq + (long)head * a.ldq_head;
             float v[F][8], top = 0.f;
@@ -120,8 +120,9 @@ template <typename T, int W, int RT> struct KvQueries {
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[f][i]));
             }
             const unsigned e = min(max(__float_as_uint(rows4_max(top)) >> 23, 1u), 253u);
-            const float down = __uint_as_float((254u - e) << 23);
-            qs[r] = a.scale * 1.4426950408889634f * __uint_as_float(e << 23);
+            // (the softmax's scale leaves its sign here, so that ``qs`` is not negative)
+            const float down = copysignf(__uint_as_float((254u - e) << 23), a.scale);
+            qs[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(e << 23);
 #pragma unroll
             for (int f = 0; f < F; ++f)
 #pragma unroll
@@ -318,7 +319,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
     const int32_t* table = a.tables + (long)b * a.ld_tables;
     if (!kv_few(a, n)) return;
 
-    for (long tile0 = (long)(part / a.splits) * ROWS; tile0 < (long)n * G; tile0 += (long)a.row_tiles * ROWS) {
+    // (rows of all heads together are below 2^31; 64 bits for the step past the end)
+    for (long first = (long)(part / a.splits) * ROWS; first < (long)n * G; first += (long)a.row_tiles * ROWS) {
+        const int tile0 = (int)first;
         KvQueries<T, W, RT> q;
         q.load(a, kvh, G, lo, n, len, tile0, qc, g);
         // ---- this workgroup's tiles of keys
@@ -414,8 +417,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
         constexpr int CG = W / 4;                           // groups of four columns
         for (int e = threadIdx.x; e < ROWS * CG; e += 256) {
             const int rr = e / CG, c = 4 * (e % CG);
-            const long row = tile0 + rr;
-            if (row >= (long)n * G) continue;
+            const int row = tile0 + rr;
+            if (row >= n * G) continue;
             float mt = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s_m[i][rr]);
@@ -470,12 +473,12 @@ __global__ __launch_bounds__(64 * NW, (W < 128 && sizeof(T) == 2 ? 3 : 2)) void 
     const int key0 = 16 * (qc >> 2) + (qc & 3), z = kv_swz<W>(key0);
     const int at_k0 = key0 * W + (((W == 32 ? g : 2 * g) ^ z) * 8), at_k1 = key0 * W + (((2 * g + 1) ^ z) * 8);
     const int at_v0 = qc * 64 + (((2 * g) ^ (qc & 7)) * 8), at_v1 = qc * 64 + (((2 * g + 1) ^ (qc & 7)) * 8);
-    const long row_tiles = ((long)n * G + ROWS - 1) / ROWS;
-    for (long i = part / a.splits; i < row_tiles; i += a.row_tiles) {
-        const long tile0 = (row_tiles - 1 - i) * ROWS, row0 = tile0 + w * 16 * RT;     // causal: the longest rows begin first
+    const int row_tiles = (n * G - 1) / ROWS + 1;
+    for (int i = part / a.splits; i < row_tiles; i += a.row_tiles) {
+        const int tile0 = (row_tiles - 1 - i) * ROWS, row0 = tile0 + w * 16 * RT;     // causal: the longest rows begin first
         KvQueries<T, W, RT> q;
         q.load(a, kvh, G, lo, n, len, row0, qc, g);
-        const int last = (int)min(tile0 + ROWS, (long)n * G) - 1, most = a.causal ? min(max(len - n + last / G + 1, 0), len) : len;
+        const int last = (int)min((long)tile0 + ROWS, (long)n * G) - 1, most = a.causal ? min(max(len - n + last / G + 1, 0), len) : len;
         const int all = (most + KV_KEYS - 1) / KV_KEYS, per = a.splits > 1 ? max((all + a.splits - 1) / a.splits, KV_MIN_TILES) : all;
         const int begin = min(split * per, all), tiles = min(begin + per, all);         // this workgroup's tiles of keys
         KvSoftmax<W, TWO> x[RT];
@@ -584,10 +587,10 @@ __global__ __launch_bounds__(64 * NW, (W < 128 && sizeof(T) == 2 ? 3 : 2)) void 
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const long row = row0 + 16 * r + qc;
+            const int row = row0 + 16 * r + qc;
             const float l = rows4_sum(x[r].l), base = x[r].m == -INFINITY ? 0.f : x[r].m;
             const float up = x[r].m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[r].m2 - base);
-            if (row >= (long)n * G) continue;
+            if (row >= n * G) continue;
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 f32x4_t y;

@@ -455,19 +455,20 @@ __device__ __forceinline__ void append_rows(const AppendSide<T>& a, const int32_
     const int sa = t0 + lane < N ? slots[t0 + lane] : -1, sb = t0 + 64 + lane < N ? slots[t0 + 64 + lane] : -1;
     const int before = t0 > 0 ? slots[t0 - 1] : -1;
     // first rows of runs among the workgroup's rows; skipped rows do not end a run
-    bool leads = false;
-    {
-        int p = __shfl_up(sa, 1, 64);
-        if (lane == 0) p = before;
-        if (lane < rows_per_wg && good(sa)) {
-            if (!good(p)) {
-                int i = t0 + lane - 2;
-                while (i >= 0 && !good(slots[i])) --i;
-                p = i >= 0 ? slots[i] : -1;
-            }
-            leads = !good(p) || p >> shift != sa >> shift;
+    int p = __shfl_up(sa, 1, 64);
+    if (lane == 0) p = before;
+    const bool mine = lane < rows_per_wg && good(sa);
+    for (unsigned long long gaps = __ballot(mine && !good(p) && t0 + lane > 0); gaps; gaps &= gaps - 1) {
+        const int at = __ffsll((long long)gaps) - 1;        // the row behind a skipped one: back to the last that was not
+        int seen = -1;
+        for (int r0 = t0 + at - 1; r0 >= 0 && seen < 0; r0 -= 64) {
+            const int s = r0 - lane >= 0 ? slots[r0 - lane] : -1;
+            const unsigned long long any = __ballot(good(s));
+            if (any) seen = __builtin_amdgcn_readlane(s, __ffsll((long long)any) - 1);
         }
+        if (lane == at) p = seen;
     }
+    const bool leads = mine && (!good(p) || p >> shift != sa >> shift);
     unsigned long long found = __ballot(leads);             // (the same in every wave)
     // few runs (chunks of prompts): teams of four waves; many (single tokens): a wave each
     const int team = nw == KV_TEAM && __popcll(found) <= 2 ? KV_TEAM : 1, rank = team > 1 ? w : 0;
@@ -492,20 +493,26 @@ __device__ __forceinline__ void append_rows(const AppendSide<T>& a, const int32_
             n = 0;
             first = block_size;
             bool more = true, order = true;
-            for (int r0 = 0; more; r0 += 64) {
-                const int r = r0 + lane, s = t + r < N ? slots[t + r] : -1;
-                const unsigned long long same = __ballot(good(s) && s >> shift == block),
-                                         other = __ballot(t + r >= N || (good(s) && s >> shift != block));
-                const unsigned long long in = other ? same & ((other & -other) - 1) : same;
-                more = !other;
-                if (in) {
-                    const int last = 63 - __clzll((long long)in);
-                    order = order && n == r0 && __ballot(lane <= last && s != s0 + r) == 0;
-                    n = r0 + last + 1;
-                    int p = (in >> lane) & 1 ? s & (block_size - 1) : block_size;
+            for (int r1 = 0; more; r1 += 256) {             // (skipped rows behind the last run are a padded batch's usual end)
+                int four[4];
 #pragma unroll
-                    for (int o = 32; o > 0; o >>= 1) p = min(p, __shfl_xor(p, o, 64));
-                    first = min(first, __builtin_amdgcn_readfirstlane(p));
+                for (int i = 0; i < 4; ++i) four[i] = t + r1 + 64 * i + lane < N ? slots[t + r1 + 64 * i + lane] : -1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r0 = r1 + 64 * i, r = r0 + lane, s = four[i];
+                    const unsigned long long same = __ballot(good(s) && s >> shift == block),
+                                             other = __ballot(t + r >= N || (good(s) && s >> shift != block));
+                    const unsigned long long in = !more ? 0 : other ? same & ((other & -other) - 1) : same;
+                    if (in) {
+                        const int last = 63 - __clzll((long long)in);
+                        order = order && n == r0 && __ballot(lane <= last && s != s0 + r) == 0;
+                        n = r0 + last + 1;
+                        int q = (in >> lane) & 1 ? s & (block_size - 1) : block_size;
+#pragma unroll
+                        for (int o = 32; o > 0; o >>= 1) q = min(q, __shfl_xor(q, o, 64));
+                        first = min(first, __builtin_amdgcn_readfirstlane(q));
+                    }
+                    more = more && !other;
                 }
             }
             straight = order;
@@ -651,6 +658,7 @@ extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_s
     if (N == 0) return ATHENA_OK;
     ATHENA_REQUIRE(d->q && d->k_codes && d->v_codes && d->k_scale && d->v_scale && d->tables && d->lens && d->out, ATHENA_E_SHAPE,
                    "athena_kv8_attention: null operand");
+    ATHENA_REQUIRE((long)N * (h / hk) < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: %d rows of %d heads are too many", N, h);
     ATHENA_REQUIRE(d->cu_rows || N == B, ATHENA_E_SHAPE, "athena_kv8_attention: %d rows for %d sequences need cu_rows", N, B);
     ATHENA_REQUIRE(athena_aligned16(d->k_codes) && athena_aligned16(d->v_codes), ATHENA_E_ALIGN,
                    "athena_kv8_attention: codes must lie on 16 bytes");

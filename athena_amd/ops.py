@@ -1333,6 +1333,8 @@ def kv_plan(lens, new_rows, tables, free_blocks, free_count, block_size, rows, i
     _int_vector("kv_plan", "free_count", free_count, 1)
     if rows < 0:
         _refuse("kv_plan", "room for %d rows", rows)
+    if in_place and lens.data_ptr() == new_rows.data_ptr():
+        _refuse("kv_plan", "lens are updated and cannot be new_rows too")
     stream = _here("kv_plan", lens, new_rows, tables, free_blocks, free_count)
     # one piece of memory for everything the plan writes afresh; what the caller does not get to see lies at its end
     sizes = [B + 1, rows, rows, 4] + ([] if in_place else [B, 1]) + [3 * B + 3]

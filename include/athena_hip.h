@@ -754,7 +754,7 @@ int athena_copy_many(const void* const* src, void* const* dst, const long* bytes
  * The cache of one attention layer, ``num_blocks`` blocks of ``block_size`` (16, 32, 64 or 128) tokens:
  *   k_codes int8 [num_blocks][hk][block_size][width]   k_scale fp32 [num_blocks][hk]
  *   v_codes int8 [num_blocks][hk][width][block_size]   v_scale fp32 [num_blocks][hk]
- * An element stands for code * scale.  width is 32, 64 or 128; heads of dk <= width columns use the first
+ * An element stands for code * scale, scales are not negative.  width is 32, 64 or 128; heads of dk <= width columns use the first
  * dk, the others hold zeros.  Codes start on 16 bytes.  Place p of the cache is token p % block_size of block
  * p / block_size; num_blocks * block_size < 2^31.
  *

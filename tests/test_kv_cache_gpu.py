@@ -215,7 +215,7 @@ def _bound(dtype, q, cache, spread, want, scale):
     dk = q.shape[2]
     scales = torch.where(torch.isfinite(cache[2]), cache[2], 0)       # (blocks with others are not visible, or give NaN)
     kmax = float((cache[0].float().abs().amax((1, 2, 3)) * scales.amax(1)).max())
-    score = float(q.double().abs().sum(-1).max()) * kmax * scale
+    score = float(q.double().abs().sum(-1).max()) * kmax * abs(scale)
     inner = 2 * 6 * math.sqrt(dk + 8) * 2.0 ** -24 * score + (2.0 ** -11 if dtype == BF16 else 2.0 ** -20)
     return torch.finfo(dtype).eps / 2 * want.abs() + inner * spread
 
@@ -580,3 +580,94 @@ def test_two_streams_at_once_give_the_same():
             outs.append(ops.kv8_attention(*args))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+# ------------------------------------------------------------------------------------------ odd calls
+@pytest.mark.parametrize("places", [[5, 4, 4, 7], [3, 3, 3], [9, 0, 15], [15, 14, 13, 12, 11, 10], [6, -1, 7, -1, -1, 8]])
+def test_append_rows_out_of_order_twice_and_with_gaps(places):
+    g = torch.Generator().manual_seed(len(places))
+    other = [32 + i for i in range(5)]                      # another block before and behind
+    slots = other[:2] + [16 + p if p >= 0 else -1 for p in places] + [48, 49] + [-1] * 300
+    k, v = (torch.randn(len(slots), 2, 40, generator=g).to(BF16) for _ in range(2))
+    got, want = _append_both(k, v, slots, _random_cache(g, 4, 2, 16, 64, 40))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_append_a_run_far_behind_skipped_rows():
+    g = torch.Generator().manual_seed(1)
+    slots = [16, 17] + [-1] * 700 + [18, 19] + [-1] * 130 + [20, 40]
+    k, v = (torch.randn(len(slots), 1, 32, generator=g) for _ in range(2))
+    got, want = _append_both(k, v, slots, _random_cache(g, 4, 1, 16, 32, 32))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_append_of_rows_that_do_not_lie_on_pairs(shift):
+    g = torch.Generator().manual_seed(shift)
+    slots = list(range(3, 40))
+    k, v = (torch.randn(37, 2, 67, generator=g).to(BF16).to(dev())[..., shift:shift + 33] for _ in range(2))
+    got, want = _append_both(k, v, slots, _random_cache(g, 4, 2, 16, 64, 33))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_append_of_broadcast_rows():
+    g = torch.Generator().manual_seed(2)
+    one = torch.randn(1, 1, 32, generator=g).to(dev()).expand(20, 2, 32)
+    got, want = _append_both(one, -one, list(range(20)), _random_cache(g, 2, 2, 16, 32, 32))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_attention_with_a_negative_scale_and_results_over_the_queries():
+    lens = [70, 33]
+    q, cache, tables, cu = _attention_case(21, lens, [1, 1], 4, 2, 64, 16, F32)
+    _check_attention(q, cache, tables, lens, cu, True, F32, scale=-0.2, one_row=True)
+    _check_attention(q, cache, tables, lens, cu, True, F32, scale=0.0, one_row=True)
+    args = [x.to(dev()) for x in (q, *cache, tables)] + [_i32(lens)]
+    want = ops.kv8_attention(*args)
+    got = ops.kv8_attention(*args, out=args[0])
+    assert got.data_ptr() == args[0].data_ptr() and torch.equal(got, want)
+
+
+def test_a_split_attention_in_two_graphs():
+    """Each recorded call has a workspace of its own: replays in turn, with eager calls between them."""
+    lens = [5000, 2500]
+    cases = [_attention_case(s, lens, [1, 1], 8, 2, 128, 64, BF16) for s in (31, 32)]
+    args = [[x.to(dev()) for x in (q, *cache, tables)] + [_i32(lens)] for q, cache, tables, _ in cases]
+    want = [ops.kv8_attention(*a) for a in args]
+    assert not torch.equal(*want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    for a in args:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(ops.kv8_attention(*a))
+        graphs.append(g)
+    for i in range(6):
+        for o in outs:
+            o.zero_()
+        for j in ((0, 1), (1, 0))[i % 2]:
+            graphs[j].replay()
+        assert torch.equal(ops.kv8_attention(*args[i % 2]), want[i % 2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), i
+
+
+def test_tensors_elsewhere_are_refused():
+    lens = [20]
+    q, cache, tables, cu = _attention_case(22, lens, [1], 2, 2, 64, 16, F32)
+    put = [x.to(dev()) for x in (q, *cache, tables)] + [_i32(lens)]
+    for i in range(len(put)):
+        mixed = list(put)
+        mixed[i] = mixed[i].cpu()
+        with pytest.raises(RuntimeError, match="current GPU"):
+            ops.kv8_attention(*mixed)
+    with pytest.raises(RuntimeError, match="current GPU"):
+        ops.kv8_append(q, put[0], _i32([0]), *put[1:5])
+    with pytest.raises(RuntimeError, match="current GPU"):
+        ops.logits_process(torch.zeros(2, 40), history=_i32([[1], [2]]))
+    same = _i32([1, 2])
+    with pytest.raises(RuntimeError, match="new_rows"):
+        ops.kv_plan(same, same, torch.zeros(2, 4, dtype=torch.int32, device=dev()), _i32([1]), _i32([1]), 16, 3)
+    with pytest.raises(TypeError, match="dtype"):
+        ops.kv8_attention(put[0].half(), *put[1:])
