@@ -611,7 +611,7 @@ static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     const long tiles = s.waves ? (most + 16 * rt * s.waves - 1) / (16 * rt * s.waves) : 0;
     s.row_tiles_many = (int)(tiles < 65536 ? tiles : 65536);
     const long pairs = (long)d->B * d->hk, units = pairs * s.row_tiles, units_many = pairs * s.row_tiles_many * (s.waves / 4);
-    const long key_tiles = ((long)d->table_width * d->block_size + KV_KEYS - 1) / KV_KEYS, cap = key_tiles / KV_MIN_TILES;
+    const long cap = (long)d->table_width * d->block_size / (KV_KEYS * KV_MIN_TILES);      // below 2048 places: 1
     long splits = s.waves ? (1535 + units_many) / units_many : (1535 + units) / units;
     if (splits > cap) splits = cap;
     s.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);

@@ -312,8 +312,8 @@ def test_attention_not_finite_inputs_stay_with_their_rows():
     q[1, 0, 3] = math.nan
     cache[3][int(tables[2, 1]), 1] = math.nan
     out = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens)).cpu()
-    nan = torch.isnan(out).any(-1)
-    assert nan.tolist() == [[False, False], [True, False], [False, True]]
+    nan = torch.isnan(out)
+    assert nan.any(-1).tolist() == [[False, False], [True, False], [False, True]] == nan.all(-1).tolist()
 
 
 def test_attention_value_scales_of_very_different_sizes():
@@ -671,3 +671,14 @@ def test_tensors_elsewhere_are_refused():
         ops.kv_plan(same, same, torch.zeros(2, 4, dtype=torch.int32, device=dev()), _i32([1]), _i32([1]), 16, 3)
     with pytest.raises(TypeError, match="dtype"):
         ops.kv8_attention(put[0].half(), *put[1:])
+
+
+@pytest.mark.parametrize("width", [1, 63, 124, 125, 127, 128, 129])
+def test_attention_with_tables_around_the_first_split(width):
+    """Tables of 16 .. 2064 places: the key axis is first divided at 2048."""
+    lens = [16 * width, 5]
+    q, cache, tables, cu = _attention_case(width, lens, [1, 1], 2, 1, 32, 16, F32)
+    assert tables.shape[1] == width
+    got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens)).cpu().double()
+    want, spread = _dense_reference(q, cache, tables, lens, cu, True, 1 / math.sqrt(32))
+    assert bool(((got - want).abs() <= _bound(F32, q, cache, spread, want, 1 / math.sqrt(32))).all())
