@@ -470,7 +470,7 @@ def _check_logits(x, kw, out=None):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("R,V,L,nb", [(1, 1, 1, 1), (3, 7, 5, 4), (2, 33, 40, 0), (10, 4233, 61, 8), (4, 8192, 300, 20),
-                                      (3, 20001, 700, 300), (2, 8200, 3, 2)])
+                                      (3, 20001, 700, 300), (2, 8200, 3, 2), (2, 150, 9, 700)])
 def test_logits(dtype, R, V, L, nb):
     x, kw = _logits_case(V, R, V, L, nb, dtype)
     _check_logits(x, kw)
