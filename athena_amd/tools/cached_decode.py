@@ -44,9 +44,13 @@ class LayerCaches:
 class CachedPropagate:
     """``time_propagate`` of a model for at most ``beam_size`` hypotheses at a time.  ``begin`` takes the encoder
     output of an utterance; each call then takes the hypotheses so far, like ``time_propagate``.  A hypothesis
-    that extends one of the call before costs one row; anything else is computed afresh."""
+    that extends one of the call before costs one row; anything else is computed afresh.
 
-    def __init__(self, model, beam_size):
+    Such a step is some thirty small launches whose shapes depend on the number of hypotheses alone (positions,
+    lengths and tables live on the GPU), so it is recorded into a HIP graph the second time a number comes up
+    (``graph`` false: never)."""
+
+    def __init__(self, model, beam_size, graph=True):
         self.model = getattr(model, "model", model)         # MtlTransformerCtc holds a SpeechTransformer
         self.layers = list(self.model.transformer.decoder.layers)
         attn = self.layers[0].attn1
@@ -54,22 +58,28 @@ class CachedPropagate:
         ops.kv8_width(self.depth)
         if beam_size < 1:
             raise ValueError("CachedPropagate: beam_size %d" % beam_size)
-        self.beam_size = int(beam_size)
+        self.beam_size, self.graph = int(beam_size), bool(graph)
         self.room = 0
         self.memory_frames = 0
         self.previous = None                                # the hypotheses of the call before, on the host
+        self.recorded = {}                                  # hypotheses -> (graph, logits); 0 after one eager step
 
     def _make_room(self, labels):
         dev, width = self.model.store.device, -(-labels // BLOCK)
         self.room = width * BLOCK
         pool = self.beam_size * width
-        self.cache = LayerCaches(len(self.layers), pool, self.heads, self.depth, dev)
+        # (one block more than there are to give: what a copy of unused table entries goes to)
+        self.cache = LayerCaches(len(self.layers), pool + 1, self.heads, self.depth, dev)
+        self.spare = pool
         self.tables = torch.full((self.beam_size, width), -1, dtype=torch.int32, device=dev)
         self.free_blocks = torch.arange(pool, dtype=torch.int32, device=dev)
         self.free_count = torch.tensor([pool], dtype=torch.int32, device=dev)
         self.lens = torch.zeros(self.beam_size, dtype=torch.int32, device=dev)
         self.done = torch.full((self.beam_size,), -1, dtype=torch.int32, device=dev)
-        self.previous = None
+        self.one = torch.ones(self.beam_size, dtype=torch.int32, device=dev)
+        self.ids = torch.zeros(self.beam_size, dtype=torch.int32, device=dev)
+        self.parents = torch.zeros(self.beam_size, dtype=torch.int64, device=dev)
+        self.previous, self.recorded = None, {}
 
     def begin(self, encoder_output, memory_mask=None, max_labels=None):
         """Projects the encoder output [1, T', d] for all layers and forgets the hypotheses of the last utterance."""
@@ -84,6 +94,8 @@ class CachedPropagate:
             self.memory = LayerCaches(len(self.layers), self.memory_frames // BLOCK, self.heads, self.depth, dev)
             self.memory_table = torch.arange(self.memory_frames // BLOCK, dtype=torch.int32, device=dev)[None]
             self.memory_slots = torch.arange(self.memory_frames, dtype=torch.int32, device=dev)
+            self.memory_lens = torch.zeros(self.beam_size, dtype=torch.int32, device=dev)
+            self.recorded = {}
         mask = AttnMask.coerce(memory_mask).key_mask
         with torch.no_grad():
             m2 = encoder_output[:1].contiguous().view(T, d)
@@ -91,9 +103,10 @@ class CachedPropagate:
             for i in range(len(self.layers)):
                 ops.kv8_append(self._split(outs[2 * i]), self._split(outs[2 * i + 1]), self.memory_slots[:T], *self.memory.of(i))
             # (the input mask hides the frames behind an utterance's end)
-            seen = torch.full((1,), T, dtype=torch.int32, device=dev) if mask is None else \
-                (mask[:1] == 0).sum(dim=1, dtype=torch.int32)
-            self.memory_lens = seen.expand(self.beam_size).contiguous()
+            if mask is None:
+                self.memory_lens.fill_(T)
+            else:
+                self.memory_lens.copy_((mask[:1] == 0).sum(dim=1, dtype=torch.int32).expand(self.beam_size))
         self.previous = None
 
     def _split(self, x):
@@ -102,15 +115,17 @@ class CachedPropagate:
     def _plan(self, n, new_rows, rows):
         return ops.kv_plan(self.lens[:n], new_rows, self.tables[:n], self.free_blocks, self.free_count, BLOCK, rows)
 
-    def _rearrange(self, parents, length):
-        """Row i goes on from what row parents[i] holds (``length`` tokens each)."""
-        n, blocks = len(parents), -(-length // BLOCK)
-        dev = self.lens.device
-        source = self.tables[torch.tensor(parents, device=dev), :blocks].reshape(-1).long()
-        contents = self.cache.copy_blocks(source)
+    def _rearrange(self, n):
+        """Row i goes on from what row ``parents[i]`` holds: everything is copied aside, all blocks are given back, and
+        the contents go into the blocks of a new plan."""
+        parents = self.parents[:n]
+        lens = self.lens.index_select(0, parents)
+        spare = lambda table: torch.where(table < 0, self.spare, table).reshape(-1).long()
+        contents = self.cache.copy_blocks(spare(self.tables.index_select(0, parents)))
         self._plan(self.beam_size, self.done, 0)
-        self._plan(n, torch.full((n,), length, dtype=torch.int32, device=dev), n * length)
-        self.cache.paste(self.tables[:n, :blocks].reshape(-1).long(), contents)
+        self.tables.fill_(-1)
+        self._plan(n, lens, n * self.room)
+        self.cache.paste(spare(self.tables[:n]), contents)
 
     def _parents(self, seqs):
         """For every hypothesis the row of the call before that it extends by one label, or None."""
@@ -128,50 +143,86 @@ class CachedPropagate:
         n, length = seqs.shape
         if not 1 <= n <= self.beam_size or self.memory_frames == 0:
             raise RuntimeError("CachedPropagate: %d hypotheses, made for 1 to %d, after begin()" % (n, self.beam_size))
-        if length > self.room:
-            raise RuntimeError("CachedPropagate: histories of %d labels, begin() made room for %d" % (length, self.room))
-        dev = self.lens.device
+        positions = self.model.store.pe(self.d_model).shape[0]
+        if length > min(self.room, positions):
+            raise RuntimeError("CachedPropagate: histories of %d labels, begin() made room for %d, the positional table for %d"
+                               % (length, self.room, positions))
         with torch.no_grad():
             self.model.store.refresh_shadows()
             parents = self._parents(seqs)
             if parents is None:                             # from the beginning
                 self._plan(self.beam_size, self.done, 0)
-                fresh, first = length, 0
+                self.tables.fill_(-1)
+                ids = torch.as_tensor(seqs).to(device=self.lens.device, dtype=torch.int32).contiguous()
+                logits = self._rows(ids.view(-1), n, length, torch.full((n,), length, dtype=torch.int32, device=self.lens.device))
             else:
-                if parents != list(range(self.previous.shape[0])):
-                    self._rearrange(parents, length - 1)
-                fresh, first = 1, length - 1
-            plan = self._plan(n, torch.full((n,), fresh, dtype=torch.int32, device=dev), n * fresh)
-            y = self._decoder(torch.as_tensor(seqs[:, first:], device=dev).to(torch.int32).contiguous(), plan, n, fresh, first)
-            last = y.view(n, fresh, self.d_model)[:, -1:].contiguous()
-            logits = self.model._project(self.model.final_layer, last)[:, -1, :].to(torch.float32)
+                self.ids[:n].copy_(torch.from_numpy(seqs[:, -1].astype(np.int32)))
+                self.parents[:n].copy_(torch.tensor(parents, dtype=torch.int64))
+                logits = self._step(n)
         self.previous = seqs.copy()
         return logits, list(history_logits) + [logits], step + 1
 
-    def _decoder(self, ids, plan, n, fresh, first):
-        """The decoder stack on the new rows ``ids`` [n, fresh], the first of them at position ``first``."""
+    def _step(self, n):
+        """One row for each of ``n`` hypotheses, from ``ids`` and ``parents``: eagerly the first time, then replayed."""
+        kept = self.recorded.get(n)
+        if kept is None:
+            self.recorded[n] = 0
+            return self._extend(n)
+        if kept == 0:
+            if not self.graph or torch.cuda.is_current_stream_capturing():
+                return self._extend(n)
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                logits = self._extend(n)
+            kept = self.recorded[n] = (graph, logits)
+        kept[0].replay()
+        return kept[1].clone()                              # (the next replay writes there again)
+
+    def _extend(self, n):
+        self._rearrange(n)
+        return self._rows(self.ids[:n], n, 1, self.one[:n])
+
+    def _rows(self, ids, n, fresh, new_rows):
+        """Logits [n, num_class] of the last of ``fresh`` new rows of every hypothesis."""
+        plan = self._plan(n, new_rows, n * fresh)
         net, M = self.model.y_net, n * fresh
         st = net.store
-        x = torch.empty((M, self.d_model), dtype=st.compute_dtype, device=ids.device)
-        ops.embed_fwd(net.embedding, ids, st.pe(self.d_model)[first:], n, fresh, self.d_model, net.num_class, net.xscale, 0.0,
-                      st.rng_state, net.site_drop, x)
-        scale = 1.0 / math.sqrt(self.depth)
-        cu = plan.cu_rows if fresh > 1 else None
+        # embedding * sqrt(d) + positional table, each row at its own position
+        x = net.embedding.index_select(0, ids.long()).mul_(net.xscale).add_(st.pe(self.d_model).index_select(0, plan.positions.long()))
+        x = x.to(st.compute_dtype)
+        scale, cu = 1.0 / math.sqrt(self.depth), plan.cu_rows if fresh > 1 else None
         table = self.memory_table.expand(n, -1)
-        x32 = None
+        x32 = qkv = None
         for i, layer in enumerate(self.layers):
-            q, k, v = lin_fwd_group([(x, M, w) for w in (layer.attn1.wq, layer.attn1.wk, layer.attn1.wv)])
+            nxt = self.layers[i + 1] if i + 1 < len(self.layers) else None
+            q, k, v = qkv if qkv is not None else lin_fwd_group([(x, M, w) for w in (layer.attn1.wq, layer.attn1.wk, layer.attn1.wv)])
             ops.kv8_append(self._split(k), self._split(v), plan.slots, *self.cache.of(i))
             a = ops.kv8_attention(self._split(q), *self.cache.of(i), self.tables[:n], self.lens[:n], cu_rows=cu, max_rows=fresh,
-                                  causal=True, scale=scale)
-            x, x32 = self._normed(x, x32, lin_fwd(a.view(M, -1), M, layer.attn1.dense)[0], layer.norm1)
-            q, _ = lin_fwd(x, M, layer.attn2.wq)
-            a = ops.kv8_attention(self._split(q), *self.memory.of(i), table, self.memory_lens[:n], cu_rows=cu, max_rows=fresh,
-                                  causal=False, scale=scale)
-            x, x32 = self._normed(x, x32, lin_fwd(a.view(M, -1), M, layer.attn2.dense)[0], layer.norm2)
-            f, _ = ffn_fwd(x, M, layer, 0.0, st.rng_state)
-            x, x32 = self._normed(x, x32, f, layer.norm3)
-        return x
+                                  causal=True, scale=scale).view(M, self.d_model)
+            tail = ops.layer_tail_ok(x, self.d_model, layer.attn1.dense) and \
+                ops.layer_tail_ok(x, self.d_model, layer.attn2.dense, layer.ffn0, layer.ffn1)
+            cross = lambda q: ops.kv8_attention(self._split(q), *self.memory.of(i), table, self.memory_lens[:n], cu_rows=cu,
+                                                max_rows=fresh, causal=False, scale=scale).view(M, self.d_model)
+            if tail:
+                # projection, residual and LayerNorm in one launch each, the next projections with them (see
+                # DecoderLayerFn); the residual stream passes on in fp32
+                t = ops.layer_tail_fwd(a, x, layer.attn1.dense, layer.norm1, None, None, None, LN_EPS, 0.0, st.rng_state, 0, 0, 0,
+                                       next_qkv=(layer.attn2.wq,), x32=x32, want_y32=True)
+                b = ops.layer_tail_fwd(cross(t["q"]), t["y1"], layer.attn2.dense, layer.norm2, layer.ffn0, layer.ffn1, layer.norm3,
+                                       LN_EPS, 0.0, st.rng_state, 0, 0, 0,
+                                       next_qkv=(nxt.attn1.wq, nxt.attn1.wk, nxt.attn1.wv) if nxt is not None else None,
+                                       x32=t["y32"], want_y32=True)
+                x, x32 = b["y2"], b["y32"]
+                qkv = (b["q"], b["k"], b["v"]) if nxt is not None else None
+                continue
+            x, x32 = self._normed(x, x32, lin_fwd(a, M, layer.attn1.dense)[0], layer.norm1)
+            x, x32 = self._normed(x, x32, lin_fwd(cross(lin_fwd(x, M, layer.attn2.wq)[0]), M, layer.attn2.dense)[0], layer.norm2)
+            x, x32 = self._normed(x, x32, ffn_fwd(x, M, layer, 0.0, st.rng_state)[0], layer.norm3)
+            qkv = None
+        last = x.view(n, fresh, self.d_model)[:, -1:].contiguous()
+        return self.model._project(self.model.final_layer, last)[:, -1, :].to(torch.float32)
 
     def _normed(self, x, x32, a, norm):
         """LayerNorm(x + a); where the kernels cover the width the residual stream passes on in fp32."""

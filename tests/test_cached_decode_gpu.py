@@ -20,14 +20,15 @@ TOL = 3e-2
 
 
 @pytest.mark.parametrize("precision", ["fp32", "bf16"])
-@pytest.mark.parametrize("mc", [model_config(32, 16, 4, 2, 2, 64), model_config(64, 16, 4, 1, 3, 96)])
-def test_cached_steps_match_the_whole_history(precision, mc):
+@pytest.mark.parametrize("graph", [True, False])
+@pytest.mark.parametrize("mc", [model_config(32, 16, 4, 2, 2, 64), model_config(64, 16, 4, 1, 3, 96), model_config(256, 16, 4, 1, 2, 512)])
+def test_cached_steps_match_the_whole_history(precision, mc, graph):
     from athena_amd import CachedPropagate
     case = dict(CASE, mc=mc)
     model, samples, _ = build(case, precision)
     ds = model.prepare_samples(_one(samples, 1))
     enc = model.model.decode(ds, None, None, return_encoder=True)
-    step = CachedPropagate(model, 3)
+    step = CachedPropagate(model, 3, graph=graph)
     step.begin(*enc, max_labels=40)
     g = np.random.default_rng(3)
     seqs = np.array([[9]])
@@ -49,6 +50,16 @@ def test_cached_steps_match_the_whole_history(precision, mc):
         want, _, _ = model.time_propagate([], torch.tensor(seqs), seqs.shape[1] - 1, enc)
         assert_close(got, want.cpu(), TOL if precision == "fp32" else 2 * TOL, "afresh")
         seqs = grow(seqs, [1, 0])
+    assert any(step.recorded.values()) == graph
+    # another utterance, the recorded steps of the first still in use
+    enc = model.model.decode(model.prepare_samples(_one(samples, 2)), None, None, return_encoder=True)
+    step.begin(*enc, max_labels=40)
+    seqs = np.array([[9]])
+    for parents in ([0, 0, 0], [2, 2, 1], [0, 1, 2]):
+        want, _, _ = model.time_propagate([], torch.tensor(seqs), seqs.shape[1] - 1, enc)
+        got, _, _ = step([], seqs, seqs.shape[1] - 1, enc)
+        assert_close(got, want.cpu(), TOL if precision == "fp32" else 2 * TOL, "next utterance, step %d" % seqs.shape[1])
+        seqs = grow(seqs, parents)
     with pytest.raises(RuntimeError):
         step([], g.integers(1, 9, size=(4, 3)), 0, enc)
     with pytest.raises(RuntimeError):
