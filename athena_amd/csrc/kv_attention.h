@@ -304,10 +304,12 @@ __device__ __forceinline__ void kv_finish(const KvAttn& a, long token, long head
 // Measured (bf16, 32 heads over 8 kv heads of 128, blocks of 64): 8 contexts of 120 to 131 K tokens 355 us for 2.07 GB,
 // 5.8 TB/s; 64 requests of 60 to 8192 tokens 115 us for 543 MB, 4.7 TB/s -- a large copy moves 4.8 TB/s here.  The smallest
 // calls (a beam of ten, a few dozen tokens) take 5.5 us, most of it the launch and the chain table -> codes -> result.
-template <typename T, int W, int RT>
+// One tile of 16 rows per wave: two (17 to 32 rows in one workgroup) spilled registers with heads of 128 and took 89 us where
+// two workgroups of one take 71 (40 rows, 32 requests of 3 to 9 K tokens), and the same time with heads of 64.
+template <typename T, int W>
 __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
     constexpr bool TWO = sizeof(T) == 4;
-    constexpr int F = W / 32, D = W / 16, ROWS = 16 * RT;
+    constexpr int RT = 1, F = W / 32, D = W / 16, ROWS = 16 * RT;
     __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_m2[4][ROWS];
     __shared__ float s_o[4][ROWS][W + 4];
     // (what is the same in all lanes of a wave is said to be, or the compiler keeps it per lane)

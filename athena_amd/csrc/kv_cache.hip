@@ -592,7 +592,7 @@ extern "C" int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_
 
 // ---------------------------------------------------------------- attention over the cache
 struct KvShape {
-    int rt, row_tiles;              // sequences of few rows: tiles of 16 rows per wave, row tiles
+    int row_tiles;                  // sequences of few rows: tiles of 16 rows
     int waves, row_tiles_many;      // sequences of many rows: waves of a workgroup (0: there are none), row tiles
     int splits;                     // shares of the key axis
 };
@@ -606,8 +606,7 @@ static constexpr int kv8_rt_many(int bytes, int width) { return bytes == 4 && wi
 static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     KvShape s;
     const long G = d->h / d->hk, most = (long)(d->cu_rows ? d->max_rows : 1) * G, few = G > KV_FEW ? G : KV_FEW, rows = most < few ? most : few;
-    s.rt = rows <= 16 || (d->dtype == ATHENA_F32 && d->width == 128) ? 1 : 2;
-    s.row_tiles = (int)((rows + 16 * s.rt - 1) / (16 * s.rt));
+    s.row_tiles = (int)((rows + 15) / 16);
     const int rt = kv8_rt_many(d->dtype == ATHENA_F32 ? 4 : 2, d->width);
     // (heads of 128: two waves fit a SIMD either way, and eight share a tile's widening, 440 against 475 us for chunks of 512 rows
     // x 4 heads behind 16 K tokens; smaller heads: three workgroups of four fit a CU and hide each other's barriers, 195 against
@@ -645,9 +644,7 @@ static void kv8_launch(KvAttn a, const KvShape& sh, hipStream_t s) {
     }
     a.row_tiles = sh.row_tiles;
     const dim3 grid((unsigned)(pairs * sh.row_tiles * sh.splits));
-    if (sh.rt == 2) {
-        if constexpr (W < 128 || sizeof(T) == 2) ATHENA_LAUNCH((kv8_attention_kernel<T, W, 2>), grid, block, 0, s, a);
-    } else ATHENA_LAUNCH((kv8_attention_kernel<T, W, 1>), grid, block, 0, s, a);
+    ATHENA_LAUNCH((kv8_attention_kernel<T, W>), grid, block, 0, s, a);
 }
 
 extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_stream_t stream) {
