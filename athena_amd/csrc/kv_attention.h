@@ -41,7 +41,7 @@ struct KvAttn {
 };
 
 #define KV_KEYS 64          // tokens of a tile
-#define KV_MIN_TILES 16     // tiles of a split at least
+#define KV_MIN_TILES 8      // tiles of a split at least
 #define KV_FEW 64           // rows of a (sequence, kv head) up to which the key axis is what is divided
 
 // eight codes as fp16: bytes b of code + 128 become 1024 + b (0x6400 | b), less 1152

@@ -602,7 +602,8 @@ static constexpr int kv8_rt_many(int bytes, int width) { return bytes == 4 && wi
 // A split costs a second launch (the join, 4 us and more) and the partial results' way out and in, so none has fewer than
 // KV_MIN_TILES tiles, and there are as many as fill the chip about three times over: 768 / 1536 / 2560 / 6000 workgroups took
 // 125 / 121 / 124 / 148 us for 64 requests of up to 8192 tokens and 358 / 361 / 366 / 385 us for 8 contexts of 131 K; of many
-// rows 1024 / 1536 / 2048 took 466 / 446 / 463 us for chunks of 512 rows behind 16 K.
+// rows 1024 / 1536 / 2048 took 466 / 446 / 463 us for chunks of 512 rows behind 16 K.  At least 16 / 8 / 4 tiles a split: 21.2 /
+// 15.8 / 14.9 us for 8 rows on 3.7 to 7.5 K tokens, 61 / 49 / 63 us for 13 chunks of 412 rows behind 1500.
 static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     KvShape s;
     const long G = d->h / d->hk, most = (long)(d->cu_rows ? d->max_rows : 1) * G, few = G > KV_FEW ? G : KV_FEW, rows = most < few ? most : few;
@@ -615,7 +616,7 @@ static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     const long tiles = s.waves ? (most + 16 * rt * s.waves - 1) / (16 * rt * s.waves) : 0;
     s.row_tiles_many = (int)(tiles < 65536 ? tiles : 65536);
     const long pairs = (long)d->B * d->hk, units = pairs * s.row_tiles, units_many = pairs * s.row_tiles_many * (s.waves / 4);
-    const long cap = (long)d->table_width * d->block_size / (KV_KEYS * KV_MIN_TILES);      // below 2048 places: 1
+    const long cap = (long)d->table_width * d->block_size / (KV_KEYS * KV_MIN_TILES);      // below 1024 places: 1
     long splits = s.waves ? (1535 + units_many) / units_many : (1535 + units) / units;
     if (splits > cap) splits = cap;
     s.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);

@@ -1429,8 +1429,8 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, tables, lens, cu_rows=N
             lens.data_ptr(), cu_rows.data_ptr() if cu_rows is not None else 0, out.data_ptr(),
             lse.data_ptr() if lse is not None else 0, ws.data_ptr() if work else 0, work, sq[0], sq[1], so[0], so[1], ldt, code, nb, bs, w,
             width, B, max_rows, n, h, hk, dk, 1 if causal else 0, scale if scale is not None else 1.0 / math.sqrt(dk), 0.0)
-        # (a table of fewer than 2048 places never needs a workspace)
-        if work or width * bs < 2048:
+        # (a table of fewer than 1024 places never needs a workspace)
+        if work or width * bs < 1024:
             break
         work = lib.athena_kv8_attention_workspace_bytes(desc)
         if not work:

@@ -809,7 +809,7 @@ int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_t stream);
  * lse: fp32 [N][h], natural logarithm of the sum of exponentials, or null.
  * ld_tables may be 0: every sequence then reads the same blocks.
  * ``workspace``: athena_kv8_attention_workspace_bytes of the same descriptor (0: none is needed; its pointers are
- * not looked at, and a table of fewer than 2048 places never needs one). */
+ * not looked at, and a table of fewer than 1024 places never needs one). */
 typedef struct {
     const void* q;
     const int8_t *k_codes, *v_codes;
