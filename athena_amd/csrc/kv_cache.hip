@@ -666,8 +666,10 @@ extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_s
     ATHENA_REQUIRE(athena_aligned16(d->k_codes) && athena_aligned16(d->v_codes), ATHENA_E_ALIGN,
                    "athena_kv8_attention: codes must lie on 16 bytes");
     const KvShape sh = kv8_shape(d);
-    ATHENA_REQUIRE(((long)B * hk + 7) / 8 * 8 * sh.row_tiles * sh.splits < (1L << 31) &&
-                       ((long)B * hk + 7) / 8 * 8 * sh.row_tiles_many * sh.splits < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: too many workgroups");
+    // (a launch has fewer than 2^32 threads)
+    const long pairs = ((long)B * hk + 7) / 8 * 8;
+    ATHENA_REQUIRE(pairs * sh.row_tiles * sh.splits < (1L << 24) && pairs * sh.row_tiles_many * sh.splits < (1L << 26) / (sh.waves ? sh.waves : 4),
+                   ATHENA_E_SHAPE, "athena_kv8_attention: too many workgroups");
     const int64_t need = athena_kv8_attention_workspace_bytes(d);
     ATHENA_REQUIRE(need == 0 || (d->workspace && d->workspace_bytes >= need), ATHENA_E_SHAPE,
                    "athena_kv8_attention: workspace of %ld bytes, %ld needed", (long)d->workspace_bytes, (long)need);

@@ -149,7 +149,7 @@ class CachedPropagate:
                                % (length, self.room, positions))
         with torch.no_grad():
             self.model.store.refresh_shadows()
-            parents = self._parents(seqs)
+            parents, self.previous = self._parents(seqs), None      # (a step that fails leaves no half history behind)
             if parents is None:                             # from the beginning
                 self._plan(self.beam_size, self.done, 0)
                 self.tables.fill_(-1)
@@ -174,7 +174,8 @@ class CachedPropagate:
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, stream=side):
+            # (other host threads, a data loader's say, may go on with calls of their own meanwhile)
+            with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
                 logits = self._extend(n)
             kept = self.recorded[n] = (graph, logits)
         kept[0].replay()

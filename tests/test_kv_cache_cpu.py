@@ -117,6 +117,18 @@ def test_the_c_entries_refuse_before_any_launch():
     assert logits(R=0) == 0 and append(n=0) == 0
 
 
+def test_attention_refuses_launches_of_too_many_threads():
+    """2^32 threads and more.  Few rows: 65535 sequences x 128 kv heads x 4 tiles of 16
+    rows are 2^25 workgroups of 256; many rows: 65528 x 8 heads x 64 tiles of 128 rows the same."""
+    lib, p = _lib.load(), 4096                          # an address that is never followed
+    attn = lambda B, h, hk, n, cu, mr: lib.athena_kv8_attention(
+        _lib.Kv8AttentionDesc.pack(p, p, p, p, p, p, p, cu, p, 0, 0, 0, h * 32, 32, h * 32, 32, 1, 0, 4, 16, 32, 1, B, mr, n, h, hk, 32, 1,
+                                   1.0, 0.0), None)
+    for call in ((65535, 8192, 128, 65535, 0, 1), (65528, 8, 8, 1 << 20, p, 8192)):
+        assert attn(*call) < 0, call
+        assert b"too many workgroups" in lib.athena_last_error(), lib.athena_last_error()
+
+
 def test_cache_width():
     assert [ops.kv8_width(n) for n in (1, 32, 33, 64, 65, 128)] == [32, 32, 64, 64, 128, 128]
     with pytest.raises(NotImplementedError):
