@@ -199,7 +199,8 @@ extern "C" int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stre
     const int bs = d->block_size;
     ATHENA_REQUIRE(bs == 16 || bs == 32 || bs == 64 || bs == 128, ATHENA_E_UNSUPPORTED,
                    "athena_kv_plan: block size %d not in {16, 32, 64, 128}", bs);
-    ATHENA_REQUIRE((long)d->table_width * bs < (1L << 31), ATHENA_E_SHAPE, "athena_kv_plan: table too wide");
+    // (steps of 64 places past the last one stay below 2^31)
+    ATHENA_REQUIRE((long)d->table_width * bs < (1L << 31) - KV_KEYS * 8, ATHENA_E_SHAPE, "athena_kv_plan: table too wide");
     ATHENA_REQUIRE(d->lens && d->new_rows && d->tables && d->free_blocks && d->free_count && d->cu_rows &&
                        ((d->slots && d->positions) || !d->rows) && d->lens_out && d->free_count_out && d->status && d->work,
                    ATHENA_E_SHAPE, "athena_kv_plan: null operand");
@@ -661,7 +662,8 @@ extern "C" int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_s
     if (N == 0) return ATHENA_OK;
     ATHENA_REQUIRE(d->q && d->k_codes && d->v_codes && d->k_scale && d->v_scale && d->tables && d->lens && d->out, ATHENA_E_SHAPE,
                    "athena_kv8_attention: null operand");
-    ATHENA_REQUIRE((long)N * (h / hk) < (1L << 31), ATHENA_E_SHAPE, "athena_kv8_attention: %d rows of %d heads are too many", N, h);
+    // (the rows of the last tile stay below 2^31)
+    ATHENA_REQUIRE((long)N * (h / hk) < (1L << 31) - 512, ATHENA_E_SHAPE, "athena_kv8_attention: %d rows of %d heads are too many", N, h);
     ATHENA_REQUIRE(d->cu_rows || N == B, ATHENA_E_SHAPE, "athena_kv8_attention: %d rows for %d sequences need cu_rows", N, B);
     ATHENA_REQUIRE(athena_aligned16(d->k_codes) && athena_aligned16(d->v_codes), ATHENA_E_ALIGN,
                    "athena_kv8_attention: codes must lie on 16 bytes");

@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void logits_process_kernel(LogitsArgs a) {
 extern "C" int athena_logits_process(const athena_logits_desc* d, athena_stream_t stream) {
     ATHENA_REQUIRE(d, ATHENA_E_SHAPE, "athena_logits_process: null descriptor");
     const int R = d->R, V = d->V;
-    ATHENA_REQUIRE(R >= 0 && R <= 65535 && V > 0 && d->L >= 0 && d->nb >= 0, ATHENA_E_SHAPE,
+    ATHENA_REQUIRE(R >= 0 && R <= 65535 && V > 0 && d->L >= 0 && d->L <= (1 << 30) && d->nb >= 0 && d->nb <= (1 << 30), ATHENA_E_SHAPE,
                    "athena_logits_process: bad shape R=%d V=%d L=%d biases=%d", R, V, d->L, d->nb);
     ATHENA_REQUIRE(d->dtype == ATHENA_F32 || d->dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_logits_process: dtype");
     if (R == 0) return ATHENA_OK;
@@ -153,9 +153,9 @@ extern "C" int athena_logits_process(const athena_logits_desc* d, athena_stream_
                     d->ld_allowed, R, V, d->history ? d->L : 0, d->nb, 0};
     const int e = d->dtype == ATHENA_BF16 ? 2 : 4;
     a.wide = athena_aligned16(d->logits) && athena_aligned16(d->out) && (R == 1 || (d->ldl * e % 16 == 0 && d->ldo * e % 16 == 0));
-    const bool large = (long)R * ((V + 4095) / 4096) >= 512;
+    const bool large = R * (((long)V + 4095) / 4096) >= 512;
     const int tile = large ? 4096 : 4096 / e;
-    const dim3 grid((V + tile - 1) / tile, R);
+    const dim3 grid((unsigned)(((long)V + tile - 1) / tile), R);
     hipStream_t s = (hipStream_t)stream;
     if (d->dtype == ATHENA_BF16) {
         if (large) ATHENA_LAUNCH((logits_process_kernel<bf16_t, 2>), grid, dim3(256), 0, s, a);

@@ -756,7 +756,7 @@ int athena_copy_many(const void* const* src, void* const* dst, const long* bytes
  *   v_codes int8 [num_blocks][hk][width][block_size]   v_scale fp32 [num_blocks][hk]
  * An element stands for code * scale, scales are not negative.  width is 32, 64 or 128; heads of dk <= width columns use the first
  * dk, the others hold zeros.  Codes start on 16 bytes.  Place p of the cache is token p % block_size of block
- * p / block_size; num_blocks * block_size < 2^31.
+ * p / block_size; num_blocks * block_size < 2^31, table_width * block_size < 2^31 - 512.
  *
  * athena_kv_plan: the blocks and places of the next new_rows[b] tokens of every request.  lens[b] tokens are
  * cached already, in the blocks tables[b * ld_tables + 0 ...] (table_width entries a request);
@@ -833,7 +833,7 @@ int athena_kv8_attention(const athena_kv8_attention_desc* d, athena_stream_t str
  *   x += bias[r * ld_bias + v] + sum of bias_values[r, j] over bias_ids[r, j] == v;
  *   -inf unless bit v % 32 of word v / 32 of allowed[r * ld_allowed + ...] is set.
  * Any of history, repetition, presence, frequency, bias, bias_ids (nb = 0), allowed may be null.  ld_bias and
- * ld_allowed may be 0 (one row for all).  out has the type of the logits and may be the logits. */
+ * ld_allowed may be 0 (one row for all).  R up to 65535, L and nb up to 2^30.  out has the type of the logits and may be the logits. */
 typedef struct {
     const void* logits;
     void* out;

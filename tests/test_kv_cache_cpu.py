@@ -95,7 +95,8 @@ def test_the_c_entries_refuse_before_any_launch():
         _lib.Kv8AttentionDesc.pack(q, codes, p, p, p, p, p, cu, p, 0, ws, 0, 128, 32, 128, 32, W, dtype, nb, bs, w, W, B, mr, n, h, 2, dk, 1,
                                    1.0, 0.0), None)
     for kw in (dict(bs=24), dict(w=48), dict(h=3), dict(dk=33), dict(dk=0), dict(dtype=2), dict(q=0), dict(nb=0), dict(B=0),
-               dict(B=70000), dict(cu=p, mr=0), dict(nb=1 << 28), dict(codes=4100), dict(n=2), dict(W=1 << 20), dict(W=1 << 27)):
+               dict(B=70000), dict(cu=p, mr=0), dict(nb=1 << 28), dict(codes=4100), dict(n=2), dict(W=1 << 20), dict(W=1 << 27),
+               dict(h=2, n=(1 << 31) - 100, cu=p)):
         assert attn(**kw) < 0, kw
         assert b"athena_kv8_attention" in lib.athena_last_error()
     assert lib.athena_kv8_attention(None, None) < 0 and lib.athena_kv8_attention_workspace_bytes(None) == 0
@@ -106,12 +107,13 @@ def test_the_c_entries_refuse_before_any_launch():
         assert b"athena_kv8_append" in lib.athena_last_error()
     plan = lambda B=1, W=4, ld=4, free=4, bs=16, rows=1, lens=p: lib.athena_kv_plan(
         _lib.KvPlanDesc.pack(lens, p, p, p, p, p, p, p, p, p, p, p, ld, W, free, B, bs, rows, 0), None)
-    for kw in (dict(B=0), dict(W=0), dict(ld=3), dict(free=0), dict(bs=20), dict(rows=-1), dict(lens=0), dict(W=1 << 27, ld=1 << 27)):
+    for kw in (dict(B=0), dict(W=0), dict(ld=3), dict(free=0), dict(bs=20), dict(rows=-1), dict(lens=0), dict(W=1 << 27, ld=1 << 27),
+               dict(W=(1 << 27) - 1, ld=1 << 27), dict(W=(1 << 24) - 1, ld=1 << 24, bs=128)):
         assert plan(**kw) < 0, kw
         assert b"athena_kv_plan" in lib.athena_last_error()
-    logits = lambda R=1, V=40, ldl=40, dtype=0, x=p, nb=0: lib.athena_logits_process(
-        _lib.LogitsDesc.pack(x, p, 0, 0, 0, 0, 0, 0, 0, 0, 0, ldl, 40, 0, 0, 0, 0, 0, dtype, R, V, 0, nb, 0), None)
-    for kw in (dict(R=-1), dict(V=0), dict(ldl=39), dict(dtype=3), dict(x=0), dict(nb=1), dict(R=70000)):
+    logits = lambda R=1, V=40, ldl=40, dtype=0, x=p, nb=0, L=0: lib.athena_logits_process(
+        _lib.LogitsDesc.pack(x, p, 0, 0, 0, 0, 0, 0, 0, 0, 0, ldl, 40, 0, 0, 0, 0, 0, dtype, R, V, L, nb, 0), None)
+    for kw in (dict(R=-1), dict(V=0), dict(ldl=39), dict(dtype=3), dict(x=0), dict(nb=1), dict(R=70000), dict(L=(1 << 30) + 1), dict(nb=(1 << 30) + 1)):
         assert logits(**kw) < 0, kw
         assert b"athena_logits_process" in lib.athena_last_error()
     assert logits(R=0) == 0 and append(n=0) == 0
