@@ -122,7 +122,10 @@ class BeamSearchDecoder:
         self.states = states
         if self.logit_rules is not None:
             logits = self.logit_rules(logits, candidate_holder.cand_seqs)
-        logprobs = torch.log_softmax(logits.to(torch.float32), dim=-1).cpu().numpy().astype(np.float32)
+        logprobs = torch.log_softmax(logits.to(torch.float32), dim=-1)
+        if self.logit_rules is not None:                   # a hypothesis that nothing may follow: not NaN, the last of all
+            logprobs = logprobs.masked_fill(logits.amax(dim=-1, keepdim=True) == -float("inf"), -float("inf"))
+        logprobs = logprobs.cpu().numpy().astype(np.float32)
         new_scores = logprobs + candidate_holder.cand_scores[:, None].astype(np.float32)
         new_states = candidate_holder.cand_states
         for scorer in self.scorers:

@@ -1,5 +1,6 @@
 """What the decoding operators refuse, checked in front of any launch (no GPU is needed), and the loop
 restatements the GPU tests compare with, checked against hand-made cases."""
+import numpy as np
 import pytest
 import torch
 
@@ -102,7 +103,7 @@ def test_the_c_entries_refuse_before_any_launch():
     assert lib.athena_kv8_attention(None, None) < 0 and lib.athena_kv8_attention_workspace_bytes(None) == 0
     append = lambda bs=16, w=32, dk=32, dtype=0, k=p, n=1, codes=p: lib.athena_kv8_append(
         _lib.Kv8AppendDesc.pack(k, p, p, codes, p, p, p, 64, 32, 64, 32, dtype, n, 4, 2, bs, dk, w, 0), None)
-    for kw in (dict(bs=8), dict(w=256), dict(dk=64), dict(dtype=5), dict(k=0), dict(n=-1), dict(codes=4097)):
+    for kw in (dict(bs=8), dict(w=256), dict(dk=64), dict(dtype=5), dict(k=0), dict(n=-1), dict(n=1 << 30), dict(codes=4097)):
         assert append(**kw) < 0, kw
         assert b"athena_kv8_append" in lib.athena_last_error()
     plan = lambda B=1, W=4, ld=4, free=4, bs=16, rows=1, lens=p: lib.athena_kv_plan(
@@ -181,3 +182,27 @@ def test_logit_rules_are_off_by_default():
     assert BeamSearchDecoder.build_decoder(hp, 4, 3, 3, lambda *a: None).logit_rules is None
     hp.frequency_penalty = 0.5
     assert BeamSearchDecoder.build_decoder(hp, 4, 3, 3, lambda *a: None).logit_rules.frequency == 0.5
+
+
+def test_a_hypothesis_that_nothing_may_follow_comes_last():
+    """Classes 0 to 3 and <eos> = 4; nothing may follow label 2, which every step likes best.  The others' scores are those
+    of the softmax, in fp32 sums of a few numbers: 1e-6."""
+    from athena_amd.tools.beam_search import BeamSearchDecoder, CandidateHolder
+    row = torch.tensor([0.0, 4.0, 5.0, 1.0, 3.0])
+
+    def step(logits, seqs, states, enc):
+        return row.expand(len(seqs), -1), list(logits), states
+
+    def rules(logits, seqs):
+        return torch.where(torch.as_tensor(seqs[:, -1:] == 2), -float("inf"), logits)
+
+    dec = BeamSearchDecoder(5, 4, 4, beam_size=2)
+    dec.decoder_one_step = step
+    dec.set_logit_rules(rules)
+    seqs = np.array([[4, 1], [4, 2]])
+    scores, _, _ = dec.beam_search_score(CandidateHolder(seqs, [], [seqs], np.zeros(2, np.float32), np.arange(2)), None)
+    want = row.double() - torch.logsumexp(row.double(), 0)
+    assert np.abs(scores[0] - want.numpy()).max() < 1e-6 and np.isneginf(scores[1]).all()
+    # alone <eos> costs 2.4; label 2 first (0.4) leads nowhere
+    out = dec(np.array([[4]]), [seqs[:1]], 0, (torch.zeros(1, 6, 8), None))[0].tolist()
+    assert out[-1] == 4 and 2 not in out
