@@ -65,7 +65,9 @@ class CachedPropagate:
         self.recorded = {}                                  # hypotheses -> (graph, logits); 0 after one eager step
 
     def _make_room(self, labels):
-        dev, width = self.model.store.device, -(-labels // BLOCK)
+        # (at least twice the room before, here and for the memory: what is recorded holds these tensors, and a row of ever longer
+        # utterances would record every step again for each of them, 3.7 ms a step where 0.55 replays them)
+        dev, width = self.model.store.device, max(-(-labels // BLOCK), 2 * self.room // BLOCK)
         self.room = width * BLOCK
         pool = self.beam_size * width
         # (one block more than there are to give: what a copy of unused table entries goes to)
@@ -79,7 +81,13 @@ class CachedPropagate:
         self.one = torch.ones(self.beam_size, dtype=torch.int32, device=dev)
         self.ids = torch.zeros(self.beam_size, dtype=torch.int32, device=dev)
         self.parents = torch.zeros(self.beam_size, dtype=torch.int64, device=dev)
-        self.previous, self.recorded = None, {}
+        self.previous = None
+        self._forget_recorded()
+
+    def _forget_recorded(self):
+        if any(self.recorded.values()):
+            torch.cuda.synchronize()                        # (the last replay may still be under way)
+        self.recorded = {}
 
     def begin(self, encoder_output, memory_mask=None, max_labels=None):
         """Projects the encoder output [1, T', d] for all layers and forgets the hypotheses of the last utterance."""
@@ -90,12 +98,12 @@ class CachedPropagate:
         if labels > self.room:
             self._make_room(labels)
         if T > self.memory_frames:
-            self.memory_frames = -(-T // BLOCK) * BLOCK
+            self.memory_frames = max(-(-T // BLOCK) * BLOCK, 2 * self.memory_frames)
             self.memory = LayerCaches(len(self.layers), self.memory_frames // BLOCK, self.heads, self.depth, dev)
             self.memory_table = torch.arange(self.memory_frames // BLOCK, dtype=torch.int32, device=dev)[None]
             self.memory_slots = torch.arange(self.memory_frames, dtype=torch.int32, device=dev)
             self.memory_lens = torch.zeros(self.beam_size, dtype=torch.int32, device=dev)
-            self.recorded = {}
+            self._forget_recorded()
         mask = AttnMask.coerce(memory_mask).key_mask
         with torch.no_grad():
             m2 = encoder_output[:1].contiguous().view(T, d)

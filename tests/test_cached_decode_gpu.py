@@ -66,6 +66,29 @@ def test_cached_steps_match_the_whole_history(precision, mc, graph):
         step([], g.integers(1, 9, size=(1, step.room + 1)), 0, enc)
 
 
+def test_longer_utterances_keep_most_of_what_is_recorded():
+    """Tolerances as above; room for 24 labels and 20 frames is 32 of each, and grows to twice that at least."""
+    from athena_amd import CachedPropagate
+    model, samples, _ = build(dict(CASE, mc=model_config(64, 16, 4, 1, 3, 96)), "fp32")
+    enc, mask = model.model.decode(model.prepare_samples(_one(samples, 1)), None, None, return_encoder=True)
+    enc = torch.cat([enc] * 8, dim=1)
+    step = CachedPropagate(model, 2)
+    seen = []
+    for T, labels, room in ((20, 24, 32), (30, 30, 32), (33, 24, 32), (40, 40, 64), (50, 64, 64), (63, 65, 128)):
+        frames = (enc[:, :T].contiguous(), None)
+        step.begin(*frames, max_labels=labels)
+        assert step.room == room and step.memory_frames == (32 if T < 33 else 64)
+        if not any(r is step.recorded for r in seen):
+            seen.append(step.recorded)
+        seqs = np.array([[9], [9]])
+        for i in range(4):
+            want, _, _ = model.time_propagate([], torch.tensor(seqs), i, frames)
+            got, _, _ = step([], seqs, i, frames)
+            assert_close(got, want.cpu(), TOL, "%d frames, step %d" % (T, i))
+            seqs = np.concatenate([seqs, [[1 + i], [2 + i]]], axis=1)
+    assert len(seen) <= 4
+
+
 def _score(p, ocfg, mem, mask, hyp):
     """Log-probability per label of a hypothesis (with its <eos>) in 64 bits."""
     sos = ocfg["num_class"] - 1
