@@ -48,7 +48,8 @@ class CachedPropagate:
 
     Such a step is some thirty small launches whose shapes depend on the number of hypotheses alone (positions,
     lengths and tables live on the GPU), so it is recorded into a HIP graph the second time a number comes up
-    (``graph`` false: never)."""
+    (``graph`` false: never).  One stream at a time: like every layer, the projections share the library's
+    workspace of the device."""
 
     def __init__(self, model, beam_size, graph=True):
         self.model = getattr(model, "model", model)         # MtlTransformerCtc holds a SpeechTransformer
