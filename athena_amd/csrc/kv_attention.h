@@ -210,7 +210,8 @@ template <int W, bool TWO> struct KvSoftmax {
     __device__ __forceinline__ void weigh_apart(f32x4_t (&s)[4], float ksq, float vs, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
         // scales that are 0 or not finite must not reach hidden keys
         const float base = m == -INFINITY ? 0.f : m, base2 = m2 == -INFINITY ? 0.f : m2;
-        float vf = vs * __builtin_amdgcn_exp2f(base - base2);
+        // (a block of zeros has scale 0; where every scale so far is 0 the power is that of the scores alone and may be infinite)
+        float vf = vs == 0.f ? 0.f : vs * __builtin_amdgcn_exp2f(base - base2);
         vf = vf > 3.4e38f ? 3.4e38f : vf;                   // (NaN stays)
 #pragma unroll
         for (int i = 0; i < 4; ++i)

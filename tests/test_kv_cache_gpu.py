@@ -682,3 +682,50 @@ def test_attention_with_tables_around_the_first_split(width):
     got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens)).cpu().double()
     want, spread = _dense_reference(q, cache, tables, lens, cu, True, 1 / math.sqrt(32))
     assert bool(((got - want).abs() <= _bound(F32, q, cache, spread, want, 1 / math.sqrt(32))).all())
+
+
+# ------------------------------------------------------------------------------------------ one key far above the others
+def _far_case(seed, lens, rows, h, hk, dk, bs, dtype, top, amp, ks, dominant_value=None):
+    """Every sequence's first token stands ``top`` (in natural units, over scores of deviation ``amp``) above the others: queries are one number
+    throughout and the first key's codes add up to it, so that sums over columns are whole numbers times a power of two and exact in fp32."""
+    q, cache, tables, cu = _attention_case(seed, lens, rows, h, hk, dk, bs, dtype)
+    kc, vc, k_scale, v_scale = cache
+    g = torch.Generator().manual_seed(seed + 1)
+    scale = 1 / math.sqrt(dk)
+    # deviation of a sum of dk codes of -n .. n: sqrt(dk n (n + 1) / 3)
+    n = 20
+    c = 2.0 ** round(math.log2(amp / (scale * ks * math.sqrt(dk * n * (n + 1) / 3))))
+    q[:] = c
+    kc[..., :dk] = torch.randint(-n, n + 1, kc[..., :dk].shape, generator=g, dtype=torch.int8)
+    k_scale[:] = ks
+    total = round(top / (c * ks * scale))
+    assert abs(total) <= 127 * dk
+    first = [int(tables[b, 0]) for b in range(len(lens))]
+    for j in range(dk):
+        kc[first, :, 0, j] = (total + j) // dk              # (adds up to ``total``)
+    if dominant_value is not None:
+        vc[first, :, :dk, 0] = dominant_value
+    return q, cache, tables, cu, scale
+
+
+# (sequences, rows, heads): single rows, whole and split key axis; a few rows; rows by the hundreds, whole and split
+FAR_SHAPES = [([64, 1000, 700], [1, 1, 1], 4, 2, 64, 16), ([20000, 64], [1, 1], 8, 2, 128, 64), ([640, 300], [5, 9], 4, 2, 32, 16),
+              ([500, 260], [300, 200], 4, 4, 64, 32), ([4001, 1000], [300, 70], 8, 2, 128, 64)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lens,rows,h,hk,dk,bs", FAR_SHAPES)
+@pytest.mark.parametrize("which", ["all", "first"])
+def test_attention_value_scales_of_zero_beside_large_scores(dtype, lens, rows, h, hk, dk, bs, which):
+    """Blocks of zeros have scale 0; a score of 120 above the others (173 in units of two) must not turn them into NaN.  Where the first key's
+    block is such a block the others' share is e^-120 and less: zero in fp32."""
+    q, cache, tables, cu, scale = _far_case(5, lens, rows, h, hk, dk, bs, dtype, 120.0, 3.0, 0.5)
+    if which == "all":
+        cache[3][:] = 0
+    else:
+        cache[3][[int(tables[b, 0]) for b in range(len(lens))]] = 0
+    one_row = max(rows) == 1
+    for causal in (True, False):
+        got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=None if one_row else _i32(cu),
+                                max_rows=max(rows), causal=causal, scale=scale)
+        assert bool((got.double().abs() < 1e-37).all()), float(got.double().abs().max())
