@@ -15,8 +15,8 @@
 //
 // Rounding.  Queries are scaled by a power of two to [1, 2) and held in fp16: bf16 queries fit (8 bits of 11; columns
 // more than 2^-17 below a row's largest lose bits), fp32 queries take two fp16 numbers (22 bits).  Probability
-// times value scale is held relative to the largest such product of its query so far (M2, beside the softmax's
-// own running maximum m): 11 bits for bf16 results, 22 bits in two numbers for fp32 results.  Sums stay in fp32.
+// times value scale is held relative to the largest such product of its query so far (see KvSoftmax):
+// 11 bits for bf16 results, 22 bits in two numbers for fp32 results.  Sums stay in fp32.
 #pragma once
 #include "common.h"
 
@@ -148,20 +148,26 @@ template <typename T, int W, int RT> struct KvQueries {
     }
 };
 
-// One tile of 16 rows: the running maxima, the sum of exponentials and the sums of values.
+// One tile of 16 rows: the running maximum m of the scores (exponents of two), the sum l of exponentials relative to 2^m, and the sums o
+// of values relative to 2^(m + unit).  ``w`` is log2 of the largest product of probability and value scale relative to m -- by itself, as
+// m + w would lose w's bits where scores are large -- and the unit its next whole number, so that changes of it are exact.
 // ``ksq`` (not negative) brings scores to exponents of two, ``vs`` is the lane's value scale, ``vl`` its logarithm to base 2.
+#define KV_NO_WEIGHT -300.f     // nothing yet; products below 2^-300 of 2^m do not show in fp32
 template <int W, bool TWO> struct KvSoftmax {
     f32x4_t o[W / 16];
-    float m, l, m2;
+    float m, l, w;
+    float lim;                  // m + unit where m is small enough for weigh(), -inf elsewhere
     __device__ __forceinline__ void begin() {
-        m = m2 = -INFINITY;
+        m = lim = -INFINITY;
+        w = KV_NO_WEIGHT;
         l = 0.f;
 #pragma unroll
         for (int d = 0; d < W / 16; ++d) o[d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
+    __device__ __forceinline__ int unit() const { return (int)ceilf(w); }
     // Steps of a tile; each is called for all of a wave's row tiles before the next, so that their chains of dependent
-    // instructions run side by side.  1: the new maxima
-    __device__ __forceinline__ void peak(f32x4_t (&s)[4], float ksq, float vl, bool whole, int seen, float& mn, float& mn2) {
+    // instructions run side by side.  1: the largest of the lane's sixteen scores
+    __device__ __forceinline__ float peak(f32x4_t (&s)[4], float ksq, bool whole, int seen) {
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -174,51 +180,56 @@ template <int W, bool TWO> struct KvSoftmax {
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][e]);
         // (a scale of 0 beside a score of -inf, which is "hidden": still hidden)
-        top = top == -INFINITY ? top : top * ksq;
-        mn = fmaxf(m, rows4_max(top));
-        mn2 = fmaxf(m2, rows4_max(top + vl));
+        return top == -INFINITY ? top : top * ksq;
     }
-    // 2: what is there already, relative to them
-    __device__ __forceinline__ void rescale(float mn, float mn2) {
-        l *= __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-        const float down = __builtin_amdgcn_exp2f(m2 - (mn2 == -INFINITY ? 0.f : mn2));
+    __device__ __forceinline__ bool grows(float top, float vl) const { return top > m || top + vl > lim; }
+    // 2, where it grows for any row: the new maxima, and what is there already relative to them.  From some size of m on a difference
+    // from it may be above 0 by a number that counts (fp32: steps of 1/16), or the sum with a scale's logarithm be too coarse (bf16: see weigh)
+    __device__ __forceinline__ void grow(float top, float vl) {
+        const float mn = fmaxf(m, rows4_max(top)), base = mn == -INFINITY ? 0.f : mn, dm = m - base;
+        const float wn = fmaxf(fmaxf(w + dm, KV_NO_WEIGHT), rows4_max(top - base + vl));
+        l *= __builtin_amdgcn_exp2f(dm);
+        const float down = __builtin_amdgcn_exp2f(dm + (ceilf(w) - ceilf(wn)));
 #pragma unroll
         for (int d = 0; d < W / 16; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[d][e] *= down;
         m = mn;
-        m2 = mn2;
+        w = wn;
+        lim = fabsf(m) < (TWO ? 1048576.f : 1024.f) ? m + ceilf(w) : -INFINITY;
     }
-    // Probability times value scale in one exponential, and the sum of the lane's sixteen divided by the scale again.
-    // Where the scale is far below the largest product so far (or 0, or not finite) that division would lose the
-    // probabilities: they are then worked out by themselves (weigh_apart).
-    __device__ __forceinline__ float shift(float vl) const { return vl + (m == -INFINITY ? 0.f : m) - (m2 == -INFINITY ? 0.f : m2); }
-    // 3: probabilities times value scales
-    __device__ __forceinline__ void weigh(f32x4_t (&s)[4], float ksq, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
-        const float at = vl - m2;
+    // 3: probabilities, their sum, and their products with the value scales, relative to the unit.
+    // fp32: by themselves.  bf16: in one exponential, and the sum of the lane's sixteen divided by the scale again.  There the exponent's
+    // constant ``at`` is rounded at the size of m (below 1024: 2^-15, results have 2^-9); the sum is divided by what is left of
+    // the scale in it (sixteen multiplications less: 474 against 488 us for chunks of 512 rows, 158 against 163 us for prompts).  Not where the value scale is 0, not finite or far from the largest product, nor where m is large.
+    __device__ __forceinline__ bool far(float vl) const { return !(fabsf(vl - lim + m) <= 40.f); }
+    __device__ __forceinline__ void weigh(f32x4_t (&s)[4], float ksq, float vs, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
+        const float vf = __builtin_ldexpf(vs, -unit()), at = TWO ? -m : vl - lim;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, at));
-                sum += s[i][e];
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, at));
+                sum += x;
+                s[i][e] = TWO ? x * vf : x;
             }
-        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift(vl)), l);
+        l = TWO ? l + sum : fmaf(sum, __builtin_amdgcn_exp2f(-(at + m)), l);
         pack(s, p, pl);
     }
-    __device__ __forceinline__ void weigh_apart(f32x4_t (&s)[4], float ksq, float vs, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
-        // scales that are 0 or not finite must not reach hidden keys
-        const float base = m == -INFINITY ? 0.f : m, base2 = m2 == -INFINITY ? 0.f : m2;
-        // (a block of zeros has scale 0; where every scale so far is 0 the power is that of the scores alone and may be infinite)
-        float vf = vs == 0.f ? 0.f : vs * __builtin_amdgcn_exp2f(base - base2);
-        vf = vf > 3.4e38f ? 3.4e38f : vf;                   // (NaN stays)
+    // the same, one after the other, for tiles with hidden keys (scales that are 0 or not finite must not reach them) and where weigh() would
+    // not do.  (A scale more than 2^126 above the unit has no probability above fp32's least number beside it: any finite factor does.)
+    __device__ __forceinline__ void weigh_apart(f32x4_t (&s)[4], float ksq, float vs, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
+        const float base = m == -INFINITY ? 0.f : m;
+        const float vf = __builtin_ldexpf(vs, vl - ceilf(w) > 126.f ? 126 - (int)ceilf(vl) : -unit());
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const bool hidden = s[i][e] == -INFINITY;
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[i][e], ksq, -base));
+                float d = fmaf(s[i][e], ksq, -base);
+                d = d > 0.f ? 0.f : d;                      // (NaN stays)
+                const float x = __builtin_amdgcn_exp2f(d);
                 l += hidden ? 0.f : x;
                 s[i][e] = hidden ? 0.f : x * vf;
             }
@@ -244,27 +255,27 @@ template <int W, bool TWO> struct KvSoftmax {
 template <typename T, int W, int RT>
 __device__ __forceinline__ void kv_weights(const KvQueries<T, W, RT>& q, KvSoftmax<W, sizeof(T) == 4> (&x)[RT], f32x4_t (&s)[RT][4], float ks,
                                            float vs, bool ok, bool whole, int j0, f16x8_t (&p)[RT][2], f16x8_t (&pl)[RT][2]) {
-    const float vl = __builtin_amdgcn_logf(fabsf(vs));      // log2
-    float mn[RT], mn2[RT];
-    bool grown = false;
+    // log2 |vs| (the instruction takes numbers below fp32's least normal one for 0)
+    const float vl = __builtin_amdgcn_logf(fabsf(__builtin_amdgcn_frexp_mantf(vs))) + (float)__builtin_amdgcn_frexp_expf(vs);
+    float top[RT];
+    bool grows = false, far = false;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        x[r].peak(s[r], ks * q.qs[r], vl, whole, ok ? q.limit[r] - j0 : 0, mn[r], mn2[r]);
-        grown = grown || mn[r] > x[r].m || mn2[r] > x[r].m2;
+        top[r] = x[r].peak(s[r], ks * q.qs[r], whole, ok ? q.limit[r] - j0 : 0);
+        grows = grows || x[r].grows(top[r], vl);
     }
-    if (__any(grown)) {
+    if (__any(grows)) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) x[r].rescale(mn[r], mn2[r]);
+        for (int r = 0; r < RT; ++r) x[r].grow(top[r], vl);
     }
-    bool far = false;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) far = far || !(x[r].shift(vl) > -40.f);
+    for (int r = 0; r < RT; ++r) far = far || x[r].far(vl);
     if (whole && !__any(far)) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) x[r].weigh(s[r], ks * q.qs[r], vl, p[r], pl[r]);
+        for (int r = 0; r < RT; ++r) x[r].weigh(s[r], ks * q.qs[r], vs, vl, p[r], pl[r]);
     } else {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) x[r].weigh_apart(s[r], ks * q.qs[r], vs, p[r], pl[r]);
+        for (int r = 0; r < RT; ++r) x[r].weigh_apart(s[r], ks * q.qs[r], vs, vl, p[r], pl[r]);
     }
 }
 
@@ -311,7 +322,8 @@ template <typename T, int W>
 __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
     constexpr bool TWO = sizeof(T) == 4;
     constexpr int RT = 1, F = W / 32, D = W / 16, ROWS = 16 * RT;
-    __shared__ float s_m[4][ROWS], s_l[4][ROWS], s_m2[4][ROWS];
+    __shared__ float s_m[4][ROWS], s_l[4][ROWS];
+    __shared__ int s_unit[4][ROWS];
     __shared__ float s_o[4][ROWS][W + 4];
     // (what is the same in all lanes of a wave is said to be, or the compiler keeps it per lane)
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, qc = lane & 15;
@@ -415,7 +427,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
             if (g == 0) {
                 s_m[w][16 * r + qc] = x[r].m;
                 s_l[w][16 * r + qc] = l;
-                s_m2[w][16 * r + qc] = x[r].m2;
+                s_unit[w][16 * r + qc] = x[r].unit();
             }
 #pragma unroll
             for (int d = 0; d < D; ++d) *(f32x4_t*)&s_o[w][16 * r + qc][16 * d + 4 * g] = x[r].o[d];
@@ -435,10 +447,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 lt += s_l[i][rr] * __builtin_amdgcn_exp2f(s_m[i][rr] - base);
-                const float up = s_m2[i][rr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m2[i][rr] - base);
+                // (2^(m - base) may be below fp32's least number where 2^(m - base + unit) is not: whole powers apart)
+                const float d = fmaxf(s_m[i][rr] - base, -1000.f), down = __builtin_amdgcn_exp2f(d - floorf(d));
+                const int power = (int)floorf(d) + s_unit[i][rr];
                 const f32x4_t z = *(const f32x4_t*)&s_o[i][rr][c];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] += z[j] * up;
+                for (int j = 0; j < 4; ++j) y[j] += __builtin_ldexpf(z[j] * down, power);
             }
             kv_finish<T>(a, lo + row / G, kvh * G + row % G, c, base, lt, y, split);
         }
@@ -601,13 +615,13 @@ __global__ __launch_bounds__(64 * NW, (W < 128 && sizeof(T) == 2 ? 3 : 2)) void 
         for (int r = 0; r < RT; ++r) {
             const int row = row0 + 16 * r + qc;
             const float l = rows4_sum(x[r].l), base = x[r].m == -INFINITY ? 0.f : x[r].m;
-            const float up = x[r].m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[r].m2 - base);
+            const int unit = x[r].unit();
             if (row >= n * G) continue;
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 f32x4_t y;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = x[r].o[d][j] * up;
+                for (int j = 0; j < 4; ++j) y[j] = __builtin_ldexpf(x[r].o[d][j], unit);
                 kv_finish<T>(a, lo + row / G, kvh * G + row % G, 16 * d + 4 * g, base, l, y, split);
             }
         }

@@ -729,3 +729,19 @@ def test_attention_value_scales_of_zero_beside_large_scores(dtype, lens, rows, h
         got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=None if one_row else _i32(cu),
                                 max_rows=max(rows), causal=causal, scale=scale)
         assert bool((got.double().abs() < 1e-37).all()), float(got.double().abs().max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lens,rows,h,hk,dk,bs", FAR_SHAPES)
+@pytest.mark.parametrize("top", [50.0, 1000.0, 2e4, 1e6, 3e7])
+def test_attention_one_key_takes_everything_in_whole_tiles(dtype, lens, rows, h, hk, dk, bs, top):
+    """The result is that key's value: two roundings of a product (2^-22 / 2^-11), whatever the size of the scores."""
+    q, cache, tables, cu, scale = _far_case(6, lens, rows, h, hk, dk, bs, dtype, top, top / 50, top / 1024)
+    got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=None if max(rows) == 1 else _i32(cu),
+                            max_rows=max(rows), causal=True, scale=scale).cpu().double()
+    first = tables[:, 0].long()
+    value = (cache[1][first][..., :dk, 0].double() * cache[3][first].double()[..., None]).repeat_interleave(h // hk, 1)
+    want = torch.cat([value[b:b + 1].expand(r, -1, -1) for b, r in enumerate(rows)])
+    tol = (torch.finfo(dtype).eps / 2 + (2.0 ** -11 if dtype == BF16 else 2.0 ** -20)) * want.abs()
+    # (at 50 the others' share is e^-45 of some thousands)
+    assert bool(((got - want).abs() <= tol + 1e-14).all()), float(((got - want).abs() / want.abs().clamp(min=1e-30)).max())
