@@ -16,7 +16,7 @@
 // Rounding.  Queries are scaled by a power of two to [1, 2) and held in fp16: bf16 queries fit (8 bits of 11; columns
 // more than 2^-17 below a row's largest lose bits), fp32 queries take two fp16 numbers (22 bits).  Probability
 // times value scale is held relative to the largest such product of its query so far (see KvSoftmax):
-// 11 bits for bf16 results, 22 bits in two numbers for fp32 results.  Sums stay in fp32.
+// 11 bits for bf16 results, 22 bits in two numbers for fp32 results, fewer far below it (KV_RAISE).  Sums stay in fp32.
 #pragma once
 #include "common.h"
 
@@ -149,9 +149,13 @@ template <typename T, int W, int RT> struct KvQueries {
 };
 
 // One tile of 16 rows: the running maximum m of the scores (exponents of two), the sum l of exponentials relative to 2^m, and the sums o
-// of values relative to 2^(m + unit).  ``w`` is log2 of the largest product of probability and value scale relative to m -- by itself, as
+// of values relative to 2^(m + unit - KV_RAISE).  ``w`` is log2 of the largest product of probability and value scale relative to m -- by itself, as
 // m + w would lose w's bits where scores are large -- and the unit its next whole number, so that changes of it are exact.
 // ``ksq`` (not negative) brings scores to exponents of two, ``vs`` is the lane's value scale, ``vl`` its logarithm to base 2.
+// Products go to the matrix units raised by 2^15, up to where fp16 ends: its numbers end at 2^-24, so that relative to a row's largest
+// product one fp16 number keeps 11 bits down to 2^-29 and something down to 2^-40, two keep 22 bits down to 2^-18 (and a bit less with
+// every further power of two).
+#define KV_RAISE 15
 #define KV_NO_WEIGHT -300.f     // nothing yet; products below 2^-300 of 2^m do not show in fp32
 template <int W, bool TWO> struct KvSoftmax {
     f32x4_t o[W / 16];
@@ -164,7 +168,7 @@ template <int W, bool TWO> struct KvSoftmax {
 #pragma unroll
         for (int d = 0; d < W / 16; ++d) o[d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ int unit() const { return (int)ceilf(w); }
+    __device__ __forceinline__ int unit() const { return (int)ceilf(w) - KV_RAISE; }     // of o
     // Steps of a tile; each is called for all of a wave's row tiles before the next, so that their chains of dependent
     // instructions run side by side.  1: the largest of the lane's sixteen scores
     __device__ __forceinline__ float peak(f32x4_t (&s)[4], float ksq, bool whole, int seen) {
@@ -204,7 +208,7 @@ template <int W, bool TWO> struct KvSoftmax {
     // the scale in it (sixteen multiplications less: 474 against 488 us for chunks of 512 rows, 158 against 163 us for prompts).  Not where the value scale is 0, not finite or far from the largest product, nor where m is large.
     __device__ __forceinline__ bool far(float vl) const { return !(fabsf(vl - lim + m) <= 40.f); }
     __device__ __forceinline__ void weigh(f32x4_t (&s)[4], float ksq, float vs, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
-        const float vf = __builtin_ldexpf(vs, -unit()), at = TWO ? -m : vl - lim;
+        const float vf = __builtin_ldexpf(vs, -unit()), at = TWO ? -m : vl + KV_RAISE - lim;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -218,10 +222,10 @@ template <int W, bool TWO> struct KvSoftmax {
         pack(s, p, pl);
     }
     // the same, one after the other, for tiles with hidden keys (scales that are 0 or not finite must not reach them) and where weigh() would
-    // not do.  (A scale more than 2^126 above the unit has no probability above fp32's least number beside it: any finite factor does.)
+    // not do.  (A scale more than 2^126 above the largest product has no probability above fp32's least number beside it: any finite factor does.)
     __device__ __forceinline__ void weigh_apart(f32x4_t (&s)[4], float ksq, float vs, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
         const float base = m == -INFINITY ? 0.f : m;
-        const float vf = __builtin_ldexpf(vs, vl - ceilf(w) > 126.f ? 126 - (int)ceilf(vl) : -unit());
+        const float vf = __builtin_ldexpf(vs, vl - ceilf(w) > 126.f ? 126 - (int)ceilf(vl) : -(int)ceilf(w));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -231,7 +235,7 @@ template <int W, bool TWO> struct KvSoftmax {
                 d = d > 0.f ? 0.f : d;                      // (NaN stays)
                 const float x = __builtin_amdgcn_exp2f(d);
                 l += hidden ? 0.f : x;
-                s[i][e] = hidden ? 0.f : x * vf;
+                s[i][e] = hidden ? 0.f : x * vf * (float)(1 << KV_RAISE);
             }
         pack(s, p, pl);
     }

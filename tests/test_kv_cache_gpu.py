@@ -745,3 +745,42 @@ def test_attention_one_key_takes_everything_in_whole_tiles(dtype, lens, rows, h,
     tol = (torch.finfo(dtype).eps / 2 + (2.0 ** -11 if dtype == BF16 else 2.0 ** -20)) * want.abs()
     # (at 50 the others' share is e^-45 of some thousands)
     assert bool(((got - want).abs() <= tol + 1e-14).all()), float(((got - want).abs() / want.abs().clamp(min=1e-30)).max())
+
+
+def _check_far(q, cache, tables, lens, cu, dtype, scale, causal, one_row, top):
+    """What is left of the bound where the sums of the scores are exact: the exponent's four roundings (the score's factor twice, the running
+    maximum, the difference), each 2^-24 of the score in units of two (1.45 top); probabilities as in ``_bound``; and products below 2^-40 of the
+    row's largest, which vanish."""
+    got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=None if one_row else _i32(cu),
+                            max_rows=max(b - a for a, b in zip(cu, cu[1:])), causal=causal, scale=scale).cpu().double()
+    want, spread = _dense_reference(q, cache, tables, lens, cu, causal, scale)
+    inner = 4 * 2.0 ** -24 * 1.45 * (top + 4) + (2.0 ** -11 if dtype == BF16 else 2.0 ** -20)
+    vmax = float((cache[1].float().abs().amax((1, 2, 3)) * cache[3].amax(1)).max())
+    err = (got - want).abs() - torch.finfo(dtype).eps / 2 * want.abs() - inner * spread - max(lens) * 2.0 ** -40 * vmax
+    assert bool((err <= 0).all()), (float(err.max()), float(((got - want).abs() / (inner * spread + 1e-300)).max()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lens,rows,h,hk,dk,bs", FAR_SHAPES)
+@pytest.mark.parametrize("top", [8.0, 10.0, 12.0, 14.0, 16.0])
+def test_attention_beside_a_key_that_dominates(dtype, lens, rows, h, hk, dk, bs, top):
+    """A first token that takes most of the mass and whose value is nothing: the result is what the others, e^-top each, come to."""
+    case = _far_case(int(top), lens, rows, h, hk, dk, bs, dtype, top, 0.5, 1 / 16, dominant_value=0)
+    for causal in (True, False):
+        _check_far(*case[:3], lens, case[3], dtype, case[4], causal, max(rows) == 1, top)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("below", [24.5, 25.1, 28.0])
+def test_attention_of_a_long_flat_tail(dtype, below):
+    """131071 equal tokens 2^-24.5 and less of the first one's weight each: 0.55 % to 0.05 % of the result together."""
+    q, cache, tables, cu, scale = _far_case(3, [131072], [1], 2, 1, 64, 64, dtype, below * math.log(2), 0.5, 1 / 16, dominant_value=100)
+    cache[0].zero_()                                        # every code 0 ...
+    first = int(tables[0, 0])
+    total = round(below * math.log(2) / (float(q[0, 0, 0]) / 16 * scale))
+    for j in range(64):
+        cache[0][first, :, 0, j] = (total + j) // 64        # ... but the first key's
+    cache[1][..., :64, :] = 90
+    cache[1][first, :, :64, 0] = 0
+    cache[3][:] = 0.013
+    _check_far(q, cache, tables, [131072], cu, dtype, scale, True, True, below * math.log(2))
