@@ -13,8 +13,8 @@
 // value scale and one table entry for its part of a tile.  The key scale multiplies scores, the value
 // scale probabilities; codes are whole numbers below 128 and exact in fp16.
 //
-// Rounding.  Queries are scaled by a power of two to [1, 2) and held in fp16: bf16 queries fit (8 bits of 11; columns
-// more than 2^-17 below a row's largest lose bits), fp32 queries take two fp16 numbers (22 bits).  Probability
+// Rounding.  Queries are scaled by a power of two to [2^14, 2^15), where fp16 ends, and held in fp16: bf16 queries fit (8 bits of 11; columns
+// more than 2^-31 below a row's largest lose bits), fp32 queries take two fp16 numbers (22 bits; fewer from 2^-17 on).  Probability
 // times value scale is held relative to the largest such product of its query so far (see KvSoftmax):
 // 11 bits for bf16 results, 22 bits in two numbers for fp32 results, fewer far below it (KV_RAISE).  Sums stay in fp32.
 #pragma once
@@ -85,7 +85,7 @@ template <int W> __device__ __forceinline__ int kv_column(int f, int g) {
     return W == 32 ? 8 * g : 64 * (f >> 1) + 16 * g + 8 * (f & 1);
 }
 
-// Queries of RT tiles of 16 rows from row ``row0`` of a (sequence, kv head), scaled by a power of two to [1, 2), as operands;
+// Queries of RT tiles of 16 rows from row ``row0`` of a (sequence, kv head), scaled by a power of two to [2^14, 2^15), as operands;
 // what the power and the softmax's scale come to (``qs``, for exponents of two); how many tokens each row sees.
 template <typename T, int W, int RT> struct KvQueries {
     static constexpr bool TWO = sizeof(T) == 4;             // fp32: queries and probabilities in two fp16 numbers
@@ -119,10 +119,11 @@ template <typename T, int W, int RT> struct KvQueries {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[f][i]));
             }
-            const unsigned e = min(max(__float_as_uint(rows4_max(top)) >> 23, 1u), 253u);
+            // (15: powers of two and their reciprocals stay normal numbers)
+            const unsigned e = min(max(__float_as_uint(rows4_max(top)) >> 23, 15u), 253u);
             // (the softmax's scale leaves its sign here, so that ``qs`` is not negative)
-            const float down = copysignf(__uint_as_float((254u - e) << 23), a.scale);
-            qs[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(e << 23);
+            const float down = copysignf(__uint_as_float((268u - e) << 23), a.scale);
+            qs[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((e - 14u) << 23);
 #pragma unroll
             for (int f = 0; f < F; ++f)
 #pragma unroll

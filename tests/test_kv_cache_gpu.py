@@ -784,3 +784,28 @@ def test_attention_of_a_long_flat_tail(dtype, below):
     cache[1][first, :, :64, 0] = 0
     cache[3][:] = 0.013
     _check_far(q, cache, tables, [131072], cu, dtype, scale, True, True, below * math.log(2))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lens,rows,h,hk,dk,bs", FAR_SHAPES)
+@pytest.mark.parametrize("small", [-14, -20, -24])
+def test_attention_queries_with_columns_of_very_different_sizes(dtype, lens, rows, h, hk, dk, bs, small):
+    """Scores made of columns 2^-14 and less of the row's largest, whose keys are zero.  A column is held to 2^-22 of itself (fp32; bf16
+    queries exactly) or 2^-39 of the largest; the rest as in ``_bound``."""
+    q, cache, tables, cu = _attention_case(11, lens, rows, h, hk, dk, bs, dtype)
+    q[..., 1:] = (q[..., 1:].float() * 2.0 ** small).to(dtype)
+    q[..., 0] = 1.5
+    cache[0][..., 0] = 0
+    cache[2][:] *= 2.0 ** -small
+    scale = 1 / math.sqrt(dk)
+    got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=None if max(rows) == 1 else _i32(cu),
+                            max_rows=max(rows), causal=True, scale=scale).cpu().double()
+    want, spread = _dense_reference(q, cache, tables, lens, cu, True, scale)
+    kmax = 127 * float(cache[2].max())
+    x = q.double().abs()
+    x[..., 0] = 0
+    held = torch.maximum(2.0 ** -22 * x, torch.tensor(2.0 ** -39 * 2).double()).sum(-1).max() if dtype == F32 else 2.0 ** -39 * 2 * dk
+    score = kmax * scale * (6 * math.sqrt(dk + 8) * 2.0 ** -24 * float(x.sum(-1).max()) + float(held))
+    inner = 2 * score + (2.0 ** -11 if dtype == BF16 else 2.0 ** -20)
+    err = (got - want).abs() - torch.finfo(dtype).eps / 2 * want.abs() - inner * spread
+    assert bool((err <= 0).all()), (float(err.max()), float(((got - want).abs() / (inner * spread)).max()))
