@@ -111,8 +111,14 @@ class BeamSearchDecoder:
         self.scorers.append(ctc_scorer)
 
     def set_logit_rules(self, rules):
-        """Penalties, biases or a grammar on the logits of every step (``LogitRules``)."""
+        """Penalties, biases or a grammar on the logits of every step (``LogitRules``).  What they leave at -inf is
+        forbidden: it is neither gone on with nor returned, however few hypotheses are left; a search whose rules let
+        no hypothesis end within the encoder's frames raises RuntimeError."""
         self.logit_rules = rules
+
+    def _allowed(self, scores):
+        """Which entries the rules leave; without rules all of them, whatever their scores."""
+        return ~np.isneginf(scores) if self.logit_rules is not None else np.ones(scores.shape, dtype=bool)
 
     def beam_search_score(self, candidate_holder, encoder_outputs):
         """One decoder step on every live hypothesis: scores [n, num_class] of extending it by each
@@ -155,21 +161,27 @@ class BeamSearchDecoder:
             n = holder.cand_seqs.shape[0]
             tiled = (enc[:1].expand(n, -1, -1), _tile_mask(enc_mask, n))
             new_scores, history, new_states = self.beam_search_score(holder, tiled)
-            done.add(holder.cand_seqs, new_scores[:, self.eos])
+            ends = self._allowed(new_scores[:, self.eos])
+            done.add(holder.cand_seqs[ends], new_scores[ends, self.eos])
             if pos + 1 >= max_seq_len:
                 break
             live = new_scores[:, open_classes]
             length = np.float32(holder.cand_seqs.shape[1] + 1)
             # every continuation is already worse than every finished hypothesis, in total and per token
-            if live.max() < done.scores.min() and (live / length).max() < done.per_token().min():
+            if len(done.scores) and live.max() < done.scores.min() and (live / length).max() < done.per_token().min():
                 break
             flat = live.reshape(-1)
             pick = _top(flat, self.beam_size) if flat.size > self.beam_size else np.arange(flat.size)
+            pick = pick[self._allowed(flat[pick])]
+            if pick.size == 0:                              # nothing may go on
+                break
             parents, syms = pick // len(open_classes), open_classes[pick % len(open_classes)]
             seqs = np.concatenate([holder.cand_seqs[parents], syms[:, None]], axis=1)
             states = [_select(s, parents) for s in new_states]
             states[0] = seqs
             holder = CandidateHolder(seqs, [_select(h, parents) for h in history], states, flat[pick], parents)
+        if len(done.scores) == 0:
+            raise RuntimeError("beam search: no hypothesis that the logit rules allow ended within %d frames" % max_seq_len)
         return torch.from_numpy(done.best()[None].astype(np.int64))
 
 

@@ -247,7 +247,8 @@ class LogitRules:
 
     ``repetition`` (> 1 makes labels of the hypothesis less likely), ``presence``, ``frequency``: see
     ``athena_logits_process``; ``bias``: {class: value}; ``grammar``: a callable that takes the hypotheses
-    [n, length] (numpy, <sos> first) and returns a bool array [n, num_class], the classes each may go on with."""
+    [n, length] (numpy, <sos> first) and returns a bool array [n, num_class], the classes each may go on with.  It is
+    asked about hypotheses that it allowed itself only; where none of them ends in time the search raises RuntimeError."""
 
     def __init__(self, repetition=1.0, presence=0.0, frequency=0.0, bias=None, grammar=None):
         if repetition <= 0:

@@ -206,3 +206,94 @@ def test_a_hypothesis_that_nothing_may_follow_comes_last():
     # alone <eos> costs 2.4; label 2 first (0.4) leads nowhere
     out = dec(np.array([[4]]), [seqs[:1]], 0, (torch.zeros(1, 6, 8), None))[0].tolist()
     assert out[-1] == 4 and 2 not in out
+
+
+# ------------------------------------------------------------------------------------------ grammars narrower than the beam
+def _search(grammar, frames, beam_size, row, ctc=None):
+    """(result, hypotheses handed to the grammar, steps) of a search over classes 0 .. n - 2 and <eos> = n - 1, every step of which likes the
+    classes as ``row`` does; ``grammar`` maps one hypothesis (a list that begins with <eos> for <sos>) to the classes it may go on with."""
+    from athena_amd.tools.beam_search import BeamSearchDecoder
+    eos, asked, steps = len(row) - 1, [], []
+
+    def step(logits, seqs, states, enc):
+        steps.append(len(seqs))
+        return torch.tensor(row).expand(len(seqs), -1), list(logits), states
+
+    def rules(logits, seqs):
+        allowed = torch.zeros(len(seqs), len(row), dtype=torch.bool)
+        for r, s in zip(allowed, seqs.tolist()):
+            asked.append(s)
+            r[list(grammar(s))] = True
+        return torch.where(allowed, logits, -float("inf"))
+
+    dec = BeamSearchDecoder(len(row), eos, eos, beam_size=beam_size)
+    dec.decoder_one_step = step
+    dec.set_logit_rules(rules)
+    start = np.array([[eos]])
+    states = [start]
+    if ctc is not None:
+        from athena_amd import CTCPrefixScorer
+        scorer = CTCPrefixScorer(eos, ctc_beam=2 * beam_size, num_classes=len(row), ctc_weight=0.3)
+        dec.set_ctc_scorer(scorer)
+        states = scorer.initial_state(states, ctc)
+    return dec(start, states, 0, (torch.zeros(1, frames, 8), None))[0].tolist(), asked, steps
+
+
+@pytest.mark.parametrize("with_ctc", [False, True])
+@pytest.mark.parametrize("beam_size", [1, 4, 10])
+def test_search_under_a_grammar_of_one_path(beam_size, with_ctc):
+    """One path of three labels and <eos>, labels that every step likes least; the search ends with it."""
+    path = [5, 0, 1, 3, 5]
+    follow = lambda s: {path[len(s)]} if s == path[:len(s)] and len(s) < 5 else set()
+    ctc = torch.log_softmax(torch.randn(1, 12, 6, generator=torch.Generator().manual_seed(1)), -1) if with_ctc else None
+    out, asked, steps = _search(follow, 12, beam_size, [-3.0, -4.0, 6.0, -5.0, 5.0, 4.0], ctc)
+    assert out == path[1:] and steps == [1, 1, 1, 1]
+    assert asked == [path[:n] for n in range(1, 5)]
+
+
+@pytest.mark.parametrize("beam_size", [2, 3, 8])
+def test_a_grammar_is_asked_about_nothing_that_it_forbade(beam_size):
+    """Even labels follow odd ones and the other way round, at most two of three; <eos> from three labels on."""
+    def follow(s):
+        if len(s) == 1:
+            return {0, 1}
+        return {c for c in (0, 1, 2) if (c + s[-1]) % 2} | ({6} if len(s) > 3 else set())
+
+    out, asked, steps = _search(follow, 9, beam_size, [1.0, 2.0, 0.5, 7.0, 6.0, 5.0, 0.0])
+    assert out[-1] == 6 and len(out) > 3
+    for s in asked + [[6] + out]:
+        assert all(c in follow(s[:i]) for i, c in enumerate(s) if i), s
+    assert max(steps) <= beam_size and steps[0] == 1
+
+
+def test_a_search_that_nothing_allowed_can_finish():
+    """No <eos> at all, and a path that is longer than the frames; in time it is found."""
+    with pytest.raises(RuntimeError, match="rules"):
+        _search(lambda s: {0, 1}, 6, 3, [1.0, 2.0, 0.0])
+    path = [3, 0, 1, 2, 0, 3]
+    follow = lambda s: {path[len(s)]} if len(s) < 6 else set()
+    with pytest.raises(RuntimeError, match="rules"):
+        _search(follow, 4, 3, [1.0, 2.0, 0.5, 0.0])
+    # (the pool of finished hypotheses is as wide as there are frames: what ends on the last one comes without its <eos>, here as without rules)
+    assert _search(follow, 5, 3, [1.0, 2.0, 0.5, 0.0])[0] == path[1:5]
+    assert _search(follow, 6, 3, [1.0, 2.0, 0.5, 0.0])[0] == path[1:]
+    with pytest.raises(RuntimeError, match="rules"):
+        _search(lambda s: set(), 6, 3, [1.0, 2.0, 0.0])
+
+
+def test_a_search_whose_rules_forbid_nothing_is_the_plain_one():
+    from athena_amd.tools.beam_search import BeamSearchDecoder
+    g = torch.Generator().manual_seed(4)
+    table = torch.randn(40, 7, generator=g) * 2
+
+    def step(logits, seqs, states, enc):
+        return table[torch.as_tensor(seqs.sum(1) % 40)], list(logits), states
+
+    for frames in (1, 2, 9):
+        outs = []
+        for rules in (None, lambda logits, seqs: logits):
+            dec = BeamSearchDecoder(7, 6, 6, beam_size=3)
+            dec.decoder_one_step = step
+            dec.set_logit_rules(rules)
+            outs.append(dec(np.array([[6]]), [np.array([[6]])], 0, (torch.zeros(1, frames, 8), None)).tolist())
+        assert outs[0] == outs[1]
