@@ -317,6 +317,18 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
             f[i][1] = to_f32<T>(e1);
         }
     };
+    // runs that are not straight: their rows one after the other, in order, with their slots; any number of skipped rows may stand between
+    auto each_row = [&](auto f) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < n; r0 += 64) {
+            const int s = r0 + lane < n ? slots[t + r0 + lane] : -1;
+#pragma unroll 1
+            for (unsigned long long left = __ballot(s >= 0 && s < slots_end); left; left &= left - 1) {
+                const int at = __ffsll((long long)left) - 1;
+                f(r0 + at, __builtin_amdgcn_readlane(s, at));
+            }
+        }
+    };
     unsigned top = 0;                                       // largest magnitude, as bits: NaN over infinity over numbers
     const auto mag = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
     if (straight) {
@@ -339,10 +351,9 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
             }
         }
     } else if (rank == 0) {
-        for (int e = lane; e < n * dk; e += 64) {
-            const int r = e / dk, s = slots[t + r];
-            if (s >= 0 && s < slots_end) top = max(top, mag(to_f32<T>(x[(long)r * a.ld_row + (e - r * dk)])));
-        }
+        each_row([&](int r, int) {
+            for (int col = lane; col < dk; col += 64) top = max(top, mag(to_f32<T>(x[(long)r * a.ld_row + col])));
+        });
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
@@ -435,15 +446,13 @@ __device__ __forceinline__ void append_run(const AppendSide<T>& a, const int32_t
             }
         }
     } else if (rank == 0) {
-        for (int r = 0; r < n; ++r) {                       // in the rows' order: of two rows for one place the later stays
-            const int s = slots[t + r];
-            if (s < 0 || s >= slots_end) continue;
+        each_row([&](int r, int s) {                        // (of two rows for one place the later stays)
             for (int col = lane; col < W; col += 64) {
                 float f = col < dk ? to_f32<T>(x[(long)r * a.ld_row + col]) : 0.f;
                 if (tiny) f = kv_lift(f, sd);
                 codes[VALUES ? col * block_size + s % block_size : (s % block_size) * W + col] = (int8_t)code_of(f, sd, inv);
             }
-        }
+        });
     }
     if (lane == 0 && rank == 0) a.scale[at] = s1;
 }

@@ -809,3 +809,22 @@ def test_attention_queries_with_columns_of_very_different_sizes(dtype, lens, row
     inner = 2 * score + (2.0 ** -11 if dtype == BF16 else 2.0 ** -20)
     err = (got - want).abs() - torch.finfo(dtype).eps / 2 * want.abs() - inner * spread
     assert bool((err <= 0).all()), (float(err.max()), float(((got - want).abs() / (inner * spread)).max()))
+
+
+def test_append_a_run_of_very_many_skipped_rows():
+    """2^24 skipped rows inside a run of heads of 128: rows times columns pass 2^31."""
+    g = torch.Generator().manual_seed(3)
+    one = torch.randn(1, 1, 128, generator=g).to(BF16)
+    n = 2 ** 24 + 3
+    slots = torch.full((n,), -1, dtype=torch.int32, device=dev())
+    slots[0], slots[n - 2], slots[n - 1] = 18, 19, 40
+    cache = _random_cache(g, 4, 1, 16, 128, 128)
+    got = [t.to(dev()) for t in cache]
+    rows = one.to(dev()).expand(n, 1, 128)
+    ops.kv8_append(rows, -rows, slots, *got)
+    few, want = one.expand(3, 1, 128), [t.clone() for t in cache]
+    ok.append(few, [18, 19, 40], want[0], want[2])
+    vt = want[1].transpose(2, 3).contiguous()
+    ok.append(-few, [18, 19, 40], vt, want[3])
+    want[1] = vt.transpose(2, 3)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
