@@ -561,7 +561,8 @@ extern "C" int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_
     const int num_blocks = d->num_blocks, hk = d->hk, block_size = d->block_size, dk = d->dk, width = d->width, N = d->N;
     int rc = kv8_check("athena_kv8_append", num_blocks, hk, block_size, dk, width);
     if (rc) return rc;
-    ATHENA_REQUIRE(N >= 0 && N < (1 << 30), ATHENA_E_SHAPE, "athena_kv8_append: N=%d (below 2^30)", N);
+    // (64 rows a workgroup of 256 threads: fewer than 2^32 threads)
+    ATHENA_REQUIRE(N >= 0 && N <= (1 << 30) - 64, ATHENA_E_SHAPE, "athena_kv8_append: N=%d (2^30 - 64 at most)", N);
     ATHENA_REQUIRE(d->dtype == ATHENA_F32 || d->dtype == ATHENA_BF16, ATHENA_E_UNSUPPORTED, "athena_kv8_append: dtype");
     if (N == 0) return ATHENA_OK;
     const void *k = d->k, *v = d->v;

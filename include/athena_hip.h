@@ -787,7 +787,7 @@ int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stream);
  * stays.  The scale of a block and head is the largest
  * magnitude written so far / 127: it only grows, and the codes in front of the new ones are then brought to
  * the grown scale (round half to even of code * old / new); a run that begins at a block's first place
- * begins the block again, whatever its scale was.  Codes are round half to even of x / scale.  A value that
+ * begins the block again, whatever its scale was.  N up to 2^30 - 64.  Codes are round half to even of x / scale.  A value that
  * is not finite makes its block's scale NaN: the block then stands for NaN until it is begun again. */
 typedef struct {
     const void *k, *v;

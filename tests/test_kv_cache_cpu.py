@@ -297,3 +297,12 @@ def test_a_search_whose_rules_forbid_nothing_is_the_plain_one():
             dec.set_logit_rules(rules)
             outs.append(dec(np.array([[6]]), [np.array([[6]])], 0, (torch.zeros(1, frames, 8), None)).tolist())
         assert outs[0] == outs[1]
+
+
+def test_append_refuses_launches_of_too_many_threads():
+    """64 rows a workgroup of 256 threads: from 2^30 - 63 rows on these are 2^32 threads."""
+    lib, p = _lib.load(), 4096                          # an address that is never followed
+    for n in ((1 << 30) - 63, (1 << 30) - 1):
+        assert -(-n // 64) * 256 >= 1 << 32
+        assert lib.athena_kv8_append(_lib.Kv8AppendDesc.pack(p, p, p, p, p, p, p, 64, 32, 64, 32, 0, n, 4, 2, 16, 32, 32, 0), None) < 0
+        assert b"N=" in lib.athena_last_error()
