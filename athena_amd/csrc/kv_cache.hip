@@ -628,7 +628,11 @@ static KvShape kv8_shape(const athena_kv8_attention_desc* d) {
     s.row_tiles_many = (int)(tiles < 65536 ? tiles : 65536);
     const long pairs = (long)d->B * d->hk, units = pairs * s.row_tiles, units_many = pairs * s.row_tiles_many * (s.waves / 4);
     const long cap = (long)d->table_width * d->block_size / (KV_KEYS * KV_MIN_TILES);      // below 1024 places: 1
-    long splits = s.waves ? (1535 + units_many) / units_many : (1535 + units) / units;
+    // (at least what N rows take however they are spread over the sequences, or a max_rows below the truth would have a workspace of
+    // hundreds of splits for all of them; as it is no call needs more than 204 MB)
+    const long wg_rows = s.waves ? 64 * rt : 16, all = d->hk * ((d->N * G + wg_rows - 1) / wg_rows), named = s.waves ? units_many : units;
+    const long work = all > named ? all : named;
+    long splits = (1535 + work) / work;
     if (splits > cap) splits = cap;
     s.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
     return s;

@@ -306,3 +306,20 @@ def test_append_refuses_launches_of_too_many_threads():
         assert -(-n // 64) * 256 >= 1 << 32
         assert lib.athena_kv8_append(_lib.Kv8AppendDesc.pack(p, p, p, p, p, p, p, 64, 32, 64, 32, 0, n, 4, 2, 16, 32, 32, 0), None) < 0
         assert b"N=" in lib.athena_last_error()
+
+
+def test_attention_workspace_of_a_row_bound_below_the_truth():
+    """``max_rows`` shapes the launch, so a call may name fewer rows than its sequences have: the workspace stays that of the rows there are."""
+    lib = _lib.load()
+    need = lambda B, mr, n, h=32, hk=8, dk=128, w=128, W=8192, bs=64, dtype=1: lib.athena_kv8_attention_workspace_bytes(
+        _lib.Kv8AttentionDesc.pack(0, 0, 0, 0, 0, 0, 0, 4096, 0, 0, 0, 0, h * dk, dk, h * dk, dk, W, dtype, 4, bs, w, W, B, mr, n, h, hk, dk, 1,
+                                   1.0, 0.0))
+    for B, n in ((1, 100000), (1, 2000000), (16, 500000), (65535, 4000000)):
+        for mr in (1, 2, 15, 17, 100, 600, 4096):
+            for dtype in (0, 1):
+                for h, hk, dk, w in ((32, 8, 128, 128), (4, 4, 64, 64), (64, 1, 128, 128), (1, 1, 24, 32)):
+                    assert need(B, mr, n, h, hk, dk, w, dtype=dtype) <= 204 << 20, (B, mr, n, h, hk)
+    # rows as they are named: splits that fill the chip about three times over, B x kv heads x tiles of 16 rows
+    assert need(64, 1, 64) == ((1535 + 512) // 512) * 64 * 32 * 129 * 4
+    assert need(8, 1, 8) == ((1535 + 64) // 64) * 8 * 32 * 129 * 4
+    assert need(1, 1, 1) == ((1535 + 8) // 8) * 32 * 129 * 4
