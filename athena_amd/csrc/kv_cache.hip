@@ -574,7 +574,11 @@ extern "C" int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_
     ATHENA_REQUIRE(athena_aligned16(k_codes) && athena_aligned16(v_codes), ATHENA_E_ALIGN, "athena_kv8_append: codes must lie on 16 bytes");
     ATHENA_REQUIRE(ldk >= 0 && ldv >= 0 && ldk < (1 << 22) && ldv < (1 << 22), ATHENA_E_SHAPE,
                    "athena_kv8_append: rows %ld / %ld elements apart (2^22 at most)", ldk, ldv);
-    const int per = (long)N * hk <= 4096 ? 1 : 64;
+    // Rows of a workgroup.  The host does not see the runs: single rows want a wave each, chunks a team per run and few workgroups that
+    // leave at once.  1 / 8 / 64 rows a workgroup, heads of 128 in bf16, blocks of 64, us: single rows 256 x 8 heads 9.6 / 11.1 / 46.8,
+    // 513 x 8 15.9 / 17.3 / 48.6, 1024 x 8 25.7 / 25.9 / 50.2, 2048 x 8 45.5 / 46.4 / 58.2; chunks of 512 rows, 512 x 4 heads
+    // 18.5 / 5.7 / 8.4, 512 x 8 20.3 / 8.1 / 8.5, 2048 x 4 35.7 / 14.3 / 8.8, 8192 x 8 237 / 81 / 28.
+    const int per = (long)N * hk <= 2048 ? 1 : (long)N * hk <= 8192 ? 8 : 64;
     const dim3 grid((N + per - 1) / per, hk, 2), block(per == 1 ? 64 : 64 * KV_TEAM);
     const long end = (long)num_blocks * block_size;
     const int shift = __builtin_ctz(block_size);

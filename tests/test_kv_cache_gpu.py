@@ -828,3 +828,24 @@ def test_append_a_run_of_very_many_skipped_rows():
     ok.append(-few, [18, 19, 40], vt, want[3])
     want[1] = vt.transpose(2, 3)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("N", [512, 513, 2047, 2048, 2049, 2200])
+def test_append_rows_of_every_workgroup_size(N):
+    """2048 and 8192 rows x heads are where the rows of a workgroup change (4 heads): single rows, short runs, long ones, gaps."""
+    g = torch.Generator().manual_seed(N)
+    bs, hk, dk = 16, 4, 32
+    blocks = torch.randperm(N // 2 + 400, generator=g).tolist()
+    slots, at = [], 0
+    while len(slots) < N:
+        kind = at % 4
+        first, n = [(at % bs, 1), (3, 9), (0, 40), (15, 2)][kind]
+        for j in range(n):
+            slots.append(blocks[at + (first + j) // bs] * bs + (first + j) % bs)
+        if kind == 1:
+            slots += [-1] * (at % 3)
+        at += (first + n - 1) // bs + 1
+    slots = slots[:N]
+    k, v = (torch.randn(N, hk, dk, generator=g).to(BF16) for _ in range(2))
+    got, want = _append_both(k, v, slots, _random_cache(g, len(blocks), hk, bs, 32, dk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
