@@ -153,6 +153,8 @@ class CachedPropagate:
         if not 1 <= n <= self.beam_size or self.memory_frames == 0:
             raise RuntimeError("CachedPropagate: %d hypotheses, made for 1 to %d, after begin()" % (n, self.beam_size))
         positions = self.model.store.pe(self.d_model).shape[0]
+        # (labels that there are not are taken for the nearest one, as time_propagate does)
+        labels = np.clip(seqs, 0, self.model.y_net.num_class - 1).astype(np.int32)
         if length > min(self.room, positions):
             raise RuntimeError("CachedPropagate: histories of %d labels, begin() made room for %d, the positional table for %d"
                                % (length, self.room, positions))
@@ -162,10 +164,10 @@ class CachedPropagate:
             if parents is None:                             # from the beginning
                 self._plan(self.beam_size, self.done, 0)
                 self.tables.fill_(-1)
-                ids = torch.as_tensor(seqs).to(device=self.lens.device, dtype=torch.int32).contiguous()
+                ids = torch.from_numpy(np.ascontiguousarray(labels)).to(self.lens.device)
                 logits = self._rows(ids.view(-1), n, length, torch.full((n,), length, dtype=torch.int32, device=self.lens.device))
             else:
-                self.ids[:n].copy_(torch.from_numpy(seqs[:, -1].astype(np.int32)))
+                self.ids[:n].copy_(torch.from_numpy(np.ascontiguousarray(labels[:, -1])))
                 self.parents[:n].copy_(torch.tensor(parents, dtype=torch.int64))
                 logits = self._step(n)
         self.previous = seqs.copy()

@@ -155,3 +155,20 @@ def test_beam_search_with_penalties_biases_and_a_grammar(kv_cache):
 
     out = decode(LogitRules(grammar=alternate))
     assert len(out) == 5 and out[-1] == eos and all((a + b) % 2 for a, b in zip([eos] + out, out[:4]))
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_labels_that_there_are_not(graph):
+    """time_propagate takes them for the nearest label; here they must not be looked up outside the table.  Tolerances as above."""
+    from athena_amd import CachedPropagate
+    model, samples, ocfg = build(dict(CASE, mc=model_config(64, 16, 4, 1, 2, 96)), "fp32")
+    enc = model.model.decode(model.prepare_samples(_one(samples, 1)), None, None, return_encoder=True)
+    step = CachedPropagate(model, 2, graph=graph)
+    step.begin(*enc, max_labels=20)
+    V = ocfg["num_class"]
+    seqs = np.array([[V - 1, -3], [V + 5, 2]])
+    for new in ([V, -1], [2 ** 30, 1], [-2 ** 31, 2 ** 31 - 1], [3, 4]):
+        want, _, _ = model.time_propagate([], torch.tensor(seqs), seqs.shape[1] - 1, enc)
+        got, _, _ = step([], seqs, seqs.shape[1] - 1, enc)
+        assert_close(got, want.cpu(), TOL, "step %d" % seqs.shape[1])
+        seqs = np.concatenate([seqs, np.array(new)[:, None]], axis=1)
