@@ -91,8 +91,15 @@ class CachedPropagate:
         self.recorded = {}
 
     def begin(self, encoder_output, memory_mask=None, max_labels=None):
-        """Projects the encoder output [1, T', d] for all layers and forgets the hypotheses of the last utterance."""
+        """Projects the encoder output [1, T', d] for all layers and forgets the hypotheses of the last utterance.
+        ``memory_mask`` hides frames behind the utterance's end only: the cache knows a length, no holes."""
         T, d = encoder_output.shape[1], encoder_output.shape[2]
+        mask, frames = AttnMask.coerce(memory_mask).key_mask, T
+        if mask is not None:
+            hidden = mask[0].cpu().numpy() != 0
+            frames = int((~hidden).sum())
+            if hidden.shape[0] != T or frames == 0 or hidden[:frames].any():
+                raise RuntimeError("CachedPropagate: the memory mask must leave the first of %d frames and hide the others" % T)
         labels = T if max_labels is None else int(max_labels)
         dev = self.model.store.device
         self.model.store.refresh_shadows()
@@ -105,17 +112,12 @@ class CachedPropagate:
             self.memory_slots = torch.arange(self.memory_frames, dtype=torch.int32, device=dev)
             self.memory_lens = torch.zeros(self.beam_size, dtype=torch.int32, device=dev)
             self._forget_recorded()
-        mask = AttnMask.coerce(memory_mask).key_mask
         with torch.no_grad():
             m2 = encoder_output[:1].contiguous().view(T, d)
             outs = lin_fwd_group([(m2, T, w) for l in self.layers for w in (l.attn2.wk, l.attn2.wv)])
             for i in range(len(self.layers)):
                 ops.kv8_append(self._split(outs[2 * i]), self._split(outs[2 * i + 1]), self.memory_slots[:T], *self.memory.of(i))
-            # (the input mask hides the frames behind an utterance's end)
-            if mask is None:
-                self.memory_lens.fill_(T)
-            else:
-                self.memory_lens.copy_((mask[:1] == 0).sum(dim=1, dtype=torch.int32).expand(self.beam_size))
+            self.memory_lens.fill_(frames)
         self.previous = None
 
     def _split(self, x):

@@ -172,3 +172,27 @@ def test_labels_that_there_are_not(graph):
         got, _, _ = step([], seqs, seqs.shape[1] - 1, enc)
         assert_close(got, want.cpu(), TOL, "step %d" % seqs.shape[1])
         seqs = np.concatenate([seqs, np.array(new)[:, None]], axis=1)
+
+
+def test_memory_masks_with_holes_are_refused():
+    """A cache has a length: what a mask leaves must be the first frames, one at least.  Tolerances as above."""
+    from athena_amd import CachedPropagate
+    model, samples, _ = build(dict(CASE, mc=model_config(64, 16, 4, 1, 2, 96)), "fp32")
+    enc, _ = model.model.decode(model.prepare_samples(_one(samples, 1)), None, None, return_encoder=True)
+    T = enc.shape[1]
+    step = CachedPropagate(model, 2)
+    for hidden in ([0], range(T), [1], [T - 2], range(1, T - 1)):
+        mask = torch.zeros(1, 1, 1, T, device=enc.device)
+        mask[..., list(hidden)] = 1
+        with pytest.raises(RuntimeError, match="mask"):
+            step.begin(enc, mask, max_labels=20)
+    with pytest.raises(RuntimeError, match="mask"):
+        step.begin(enc, torch.zeros(1, 1, 1, T - 1, device=enc.device), max_labels=20)
+    for frames in (1, T - 1, T):
+        mask = torch.zeros(1, 1, 1, T, device=enc.device)
+        mask[..., frames:] = 1
+        step.begin(enc, mask, max_labels=20)
+        seqs = np.array([[9, 1], [9, 2]])
+        want, _, _ = model.time_propagate([], torch.tensor(seqs), 1, (enc, mask))
+        got, _, _ = step([], seqs, 1, (enc, mask))
+        assert_close(got, want.cpu(), TOL, "%d frames" % frames)
