@@ -319,8 +319,8 @@ __device__ __forceinline__ void kv_finish(const KvAttn& a, long token, long head
 // The four waves of a workgroup take every fourth tile of its share of the keys and meet once, at the end; a lane's codes go
 // from memory straight into operands, one tile ahead of their use (two waves per SIMD keep 64 KB of a CU's loads under way).
 // Measured (bf16, 32 heads over 8 kv heads of 128, blocks of 64): 8 contexts of 120 to 131 K tokens 355 us for 2.07 GB,
-// 5.8 TB/s; 64 requests of 60 to 8192 tokens 115 us for 543 MB, 4.7 TB/s -- a large copy moves 4.8 TB/s here.  The smallest
-// calls (a beam of ten, a few dozen tokens) take 5.5 us, most of it the launch and the chain table -> codes -> result.
+// 5.8 TB/s; 64 requests of 60 to 8192 tokens 116 us for 543 MB, 4.7 TB/s (fp32 118 us) -- a large copy moves 4.8 TB/s here.  The
+// smallest calls (a beam of ten, a few dozen tokens) take 6.2 us, most of it the launch and the chain table -> codes -> result.
 // One tile of 16 rows per wave: two (17 to 32 rows in one workgroup) spilled registers with heads of 128 and took 89 us where
 // two workgroups of one take 71 (40 rows, 32 requests of 3 to 9 K tokens), and the same time with heads of 64.
 template <typename T, int W>
@@ -469,11 +469,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(KvAttn a) {
 // A wave owns 16 RT rows, the NW waves of a workgroup walk its share of the keys together: a tile is loaded once (each thread a few
 // 16-byte pieces), widened once and left in LDS as fp16, double-buffered, one barrier a tile.  Widening took more
 // vector instructions than the softmax when every wave did it for itself.
-// Measured (bf16, causal): chunks of 128 to 512 rows x 4 heads behind 2 to 16 K tokens (heads of 128) 430 us for 269 GFLOP, 626
-// TFLOP/s, and 23 us for the join of three splits; three prompts of 1501 to 4001 rows, 16 heads of 64, 143 us for 68.7 GFLOP, 480
-// TFLOP/s.  A large library product reaches 1330 TFLOP/s.  What bounds it: 16 rows x 64 keys are 180 vector instructions, 32 of
-// them exponentials and the like at a quarter rate (about 900 clocks with heads of 128), beside 512 clocks of matrix instructions,
-// and two or three waves per SIMD overlap them in part only (matrix units busy 24 % of the time, waves waiting 30 %).
+// Measured (bf16, causal): chunks of 128 to 512 rows x 4 heads behind 2 to 16 K tokens (heads of 128) 403 us for 269 GFLOP, 668
+// TFLOP/s, and 22 us for the join of three splits; three prompts of 1501 to 4001 rows, 16 heads of 64, 148 us for 68.7 GFLOP, 464
+// TFLOP/s.  fp32 (two fp16 numbers each) 649 and 217 us.  A large library product reaches 1330 TFLOP/s.  What bounds it: 16 rows x 64
+// keys are 175 vector instructions, 16 of them exponentials at a quarter rate, beside 512 clocks of matrix instructions (heads of 128),
+// and two or three waves per SIMD overlap them in part only (vector units busy 47 % of the time, matrix units 26 %, waves waiting 30 %;
+// prompts 68, 19 and 30 %).
 // LDS images in 16-byte chunks (8 numbers), placed so that the 8 lanes that read side by side hit 8 different groups of
 // banks: keys [64][W], chunk ^ swz(key); values [W][64], chunk ^ (column & 7).
 template <int W> __device__ __forceinline__ int kv_swz(int key) {
@@ -635,7 +636,7 @@ __global__ __launch_bounds__(64 * NW, (W < 128 && sizeof(T) == 2 ? 3 : 2)) void 
 
 // out = the splits' results weighted by their share of the sum of exponentials; one wave per (row, head).  Bound by the
 // latency of its loads: the weights are worked out by the lanes side by side, the results then requested eight at a time
-// (24 splits of 256 rows 5.7 us; 27 us with one request after the other).
+// (24 splits of 256 rows 6.4 us; 27 us with one request after the other).
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttn a) {
     const int lane = threadIdx.x & 63, head = blockIdx.y * 4 + (threadIdx.x >> 6), b = blockIdx.z;

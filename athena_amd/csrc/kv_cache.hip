@@ -14,8 +14,8 @@
 // One workgroup sums over the requests (new rows, blocks taken, blocks given back), decides whether the
 // plan fits, and leaves the running sums; rows, table entries and returned blocks are then filled in by
 // ``plan_fill``, in the same workgroup or in a launch of many.  Whole numbers throughout.
-// Bound by latency: 16 requests 5.9 us in one launch; 2048 requests, half of them giving back some 250 blocks each, 11.8 K new
-// rows 6.7 + 6.1 us in two (318 us when one workgroup filled them; 8.2 us for the filling when a row searched for its request
+// Bound by latency: 16 requests 6.0 us in one launch; 2048 requests, half of them giving back some 250 blocks each, 11.8 K new
+// rows 6.8 + 7.0 us in two (318 us when one workgroup filled them; 8.2 us for the filling when a row searched for its request
 // instead of a request's wave laying out its rows).
 #define PLAN_THREADS 1024
 
@@ -234,7 +234,8 @@ extern "C" int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stre
 //
 // A lane holds two columns of 16 consecutive places, so that the values' codes (16 bytes of one column) leave
 // in one store.  Bound by latency: slots -> rows -> largest magnitude -> codes is a chain of four trips to memory, about 5 us a
-// run.  8192 rows of 8 heads of 128 in bf16 26 us (50 MB, 1.9 TB/s), 256 single rows 10 us.
+// run.  8192 rows of 8 heads of 128 in bf16 26 us (50 MB, 1.9 TB/s; fp32 31 us), 256 single rows 9.8 us, ten of 4 heads of 64 4.9 us.
+// Where every run makes its block's scale grow, 35 and 25 us: the codes in front of it are read and written again, four at a time.
 template <typename T> struct AppendSide {
     const T* x;
     long ld_row, ld_head;

@@ -67,7 +67,7 @@ class CachedPropagate:
 
     def _make_room(self, labels):
         # (at least twice the room before, here and for the memory: what is recorded holds these tensors, and a row of ever longer
-        # utterances would record every step again for each of them, 3.7 ms a step where 0.55 replays them)
+        # utterances would make new ones and record every step again for each of them: recording alone 0.7 ms a step of 40, replays 0.56)
         dev, width = self.model.store.device, max(-(-labels // BLOCK), 2 * self.room // BLOCK)
         self.room = width * BLOCK
         pool = self.beam_size * width

@@ -770,7 +770,7 @@ int athena_copy_many(const void* const* src, void* const* dst, const long* bytes
  * requests with a negative length or longer than their table, rows missing, returned blocks beyond
  * free_capacity}.  A plan that does not fit leaves a status that is not zero and changes nothing: no rows
  * (cu_rows 0, slots -1), lens_out = lens, free_count_out = free_count.  ``work``: int32 [3 * B + 3].
- * A block belongs to one request. */
+ * A block belongs to one request; B at least 1. */
 typedef struct {
     const int32_t *lens, *new_rows;
     int32_t *tables, *free_blocks;
@@ -787,8 +787,9 @@ int athena_kv_plan(const athena_kv_plan_desc* d, athena_stream_t stream);
  * stays.  The scale of a block and head is the largest
  * magnitude written so far / 127: it only grows, and the codes in front of the new ones are then brought to
  * the grown scale (round half to even of code * old / new); a run that begins at a block's first place
- * begins the block again, whatever its scale was.  N up to 2^30 - 64.  Codes are round half to even of x / scale.  A value that
- * is not finite makes its block's scale NaN: the block then stands for NaN until it is begun again. */
+ * begins the block again, whatever its scale was.  Codes are round half to even of x / scale.  A value that
+ * is not finite makes its block's scale NaN: the block then stands for NaN until it is begun again.
+ * N up to 2^30 - 64; ldk and ldv 0 to 2^22 - 1, hk up to 65535. */
 typedef struct {
     const void *k, *v;
     const int32_t* slots;
@@ -805,7 +806,12 @@ int athena_kv8_append(const athena_kv8_append_desc* d, athena_stream_t stream);
  * n sees the tokens j <= lens[b] - n + i.  Query head i reads kv head i / (h / hk).  A row that sees nothing
  * gives zeros (lse -inf).  Table entries outside [0, num_blocks) hold no tokens; lengths are cut at
  * table_width * block_size, rows at N; rows that belong to no sequence are left as they were.
- * max_rows: the largest number of rows of a sequence (it shapes the launch; results do not depend on it).
+ * max_rows: the largest number of rows of a sequence (it shapes the launch and the workspace; a number below the truth makes the call
+ * slower, results differ by the order of their sums only).
+ * Rounding, besides that of the result: scores and sums in fp32; queries in fp16 (fp32 queries in two such numbers) raised so that
+ * columns down to 2^-31 of a row's largest keep a bf16 number's bits and fp32 ones 22 bits down to 2^-17; probability times value
+ * scale, relative to the row's largest, in 11 bits down to 2^-29 (fp32 queries: 22 down to 2^-18), fewer further down and
+ * nothing below 2^-40.
  * lse: fp32 [N][h], natural logarithm of the sum of exponentials, or null.
  * ld_tables may be 0: every sequence then reads the same blocks.
  * ``workspace``: athena_kv8_attention_workspace_bytes of the same descriptor (0: none is needed; its pointers are
