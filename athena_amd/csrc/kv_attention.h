@@ -150,8 +150,8 @@ template <typename T, int W, int RT> struct KvQueries {
 };
 
 // One tile of 16 rows: the running maximum m of the scores (exponents of two), the sum l of exponentials relative to 2^m, and the sums o
-// of values relative to 2^(m + unit - KV_RAISE).  ``w`` is log2 of the largest product of probability and value scale relative to m -- by itself, as
-// m + w would lose w's bits where scores are large -- and the unit its next whole number, so that changes of it are exact.
+// of values relative to 2^(m + unit()).  ``w`` is log2 of the largest product of probability and value scale relative to m -- by itself,
+// as m + w would lose w's bits where scores are large; the unit is made of its next whole number, so that changes of it are exact.
 // ``ksq`` (not negative) brings scores to exponents of two, ``vs`` is the lane's value scale, ``vl`` its logarithm to base 2.
 // Products go to the matrix units raised by 2^15, up to where fp16 ends: its numbers end at 2^-24, so that relative to a row's largest
 // product one fp16 number keeps 11 bits down to 2^-29 and something down to 2^-40, two keep 22 bits down to 2^-18 (and a bit less with
@@ -161,7 +161,7 @@ template <typename T, int W, int RT> struct KvQueries {
 template <int W, bool TWO> struct KvSoftmax {
     f32x4_t o[W / 16];
     float m, l, w;
-    float lim;                  // m + unit where m is small enough for weigh(), -inf elsewhere
+    float lim;                  // m + ceil(w) where m is small enough for weigh(), -inf elsewhere
     __device__ __forceinline__ void begin() {
         m = lim = -INFINITY;
         w = KV_NO_WEIGHT;
@@ -205,8 +205,9 @@ template <int W, bool TWO> struct KvSoftmax {
     }
     // 3: probabilities, their sum, and their products with the value scales, relative to the unit.
     // fp32: by themselves.  bf16: in one exponential, and the sum of the lane's sixteen divided by the scale again.  There the exponent's
-    // constant ``at`` is rounded at the size of m (below 1024: 2^-15, results have 2^-9); the sum is divided by what is left of
-    // the scale in it (sixteen multiplications less: 474 against 488 us for chunks of 512 rows, 158 against 163 us for prompts).  Not where the value scale is 0, not finite or far from the largest product, nor where m is large.
+    // constant ``at`` is rounded at the size of m (below 1024: by 2^-14, results have 2^-9); the sum is divided by what is left of
+    // the scale in it (sixteen multiplications less: 474 against 488 us for chunks of 512 rows, 158 against 163 us for prompts).
+    // Not where the value scale is 0, not finite or far from the largest product, nor where m is large.
     __device__ __forceinline__ bool far(float vl) const { return !(fabsf(vl - lim + m) <= 40.f); }
     __device__ __forceinline__ void weigh(f32x4_t (&s)[4], float ksq, float vs, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
         const float vf = __builtin_ldexpf(vs, -unit()), at = TWO ? -m : vl + KV_RAISE - lim;
@@ -223,7 +224,8 @@ template <int W, bool TWO> struct KvSoftmax {
         pack(s, p, pl);
     }
     // the same, one after the other, for tiles with hidden keys (scales that are 0 or not finite must not reach them) and where weigh() would
-    // not do.  (A scale more than 2^126 above the largest product has no probability above fp32's least number beside it: any finite factor does.)
+    // not do.  (A scale more than 2^126 above the largest product has no probability above fp32's least number beside it: any finite factor
+    // does.)
     __device__ __forceinline__ void weigh_apart(f32x4_t (&s)[4], float ksq, float vs, float vl, f16x8_t (&p)[2], f16x8_t (&pl)[2]) {
         const float base = m == -INFINITY ? 0.f : m;
         const float vf = __builtin_ldexpf(vs, vl - ceilf(w) > 126.f ? 126 - (int)ceilf(vl) : -(int)ceilf(w));

@@ -849,3 +849,22 @@ def test_append_rows_of_every_workgroup_size(N):
     k, v = (torch.randn(N, hk, dk, generator=g).to(BF16) for _ in range(2))
     got, want = _append_both(k, v, slots, _random_cache(g, len(blocks), hk, bs, 32, dk))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("top", [-700.0, -100.0, 300.0, 700.0])
+@pytest.mark.parametrize("lens,rows,h,hk,dk,bs", FAR_SHAPES)
+def test_attention_of_large_scores_in_one_exponential(lens, rows, h, hk, dk, bs, top):
+    """bf16 below 1024 in units of two, where a score and a value scale's logarithm meet in one number: twice 2^-14 of an exponent is 8.5e-5
+    of a term, within the 2^-11 of ``_bound``; so are scores that are all far below 0 (one key above the others takes everything).  Products
+    below 2^-40 of the row's largest vanish, as in ``_check_far``: where the first value is 0, what is left are the others', e^-100 and less."""
+    q, cache, tables, cu, scale = _far_case(8, lens, rows, h, hk, dk, bs, BF16, abs(top), abs(top) / 50, abs(top) / 1024)
+    if top < 0:
+        cache[0][..., :dk] = (cache[0][..., :dk].int() // 16 - 40).to(torch.int8)
+        first = [int(tables[b, 0]) for b in range(len(lens))]
+        cache[0][first, :, 0, :dk] = -30
+    got = ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens), cu_rows=None if max(rows) == 1 else _i32(cu),
+                            max_rows=max(rows), causal=True, scale=scale).cpu().double()
+    want, spread = _dense_reference(q, cache, tables, lens, cu, True, scale)
+    vmax = float((cache[1].float().abs().amax((1, 2, 3)) * cache[3].amax(1)).max())
+    tol = _bound(BF16, q, cache, spread, want, scale) + max(lens) * 2.0 ** -40 * vmax
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol.clamp(min=1e-30)).max())
