@@ -868,3 +868,25 @@ def test_attention_of_large_scores_in_one_exponential(lens, rows, h, hk, dk, bs,
     vmax = float((cache[1].float().abs().amax((1, 2, 3)) * cache[3].amax(1)).max())
     tol = _bound(BF16, q, cache, spread, want, scale) + max(lens) * 2.0 ** -40 * vmax
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol.clamp(min=1e-30)).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("lens,rows,h,hk,dk,bs", FAR_SHAPES)
+def test_attention_scales_that_are_not_finite_in_whole_tiles(dtype, which, lens, rows, h, hk, dk, bs):
+    """Rows that see such a block are NaN, those in front of it and the other kv heads are what they were, to the bit."""
+    q, cache, tables, cu = _attention_case(14, lens, rows, h, hk, dk, bs, dtype)
+    call = lambda: ops.kv8_attention(q.to(dev()), *[x.to(dev()) for x in cache], tables.to(dev()), _i32(lens),
+                                     cu_rows=None if max(rows) == 1 else _i32(cu), max_rows=max(rows)).cpu()
+    want = call()
+    hit = [(n - r // 2 - 1) // bs for n, r in zip(lens, rows)]
+    for b, j in enumerate(hit):
+        cache[which][int(tables[b, j]), hk - 1] = math.nan
+    got = call()
+    for b, (n, r) in enumerate(zip(lens, rows)):
+        sees = torch.arange(n - r, n) >= hit[b] * bs
+        nan = torch.zeros(r, h, dtype=torch.bool)
+        nan[sees, h - h // hk:] = True
+        part = got[cu[b]:cu[b + 1]]
+        assert torch.equal(torch.isnan(part).any(-1), nan) and torch.equal(torch.isnan(part).all(-1), nan)
+        assert torch.equal(part[~nan], want[cu[b]:cu[b + 1]][~nan])
